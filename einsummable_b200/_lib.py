@@ -60,6 +60,35 @@ class es_attention_t(ctypes.Structure):
                 ("mask_stride", ctypes.c_int64)]
 
 
+class es_paged_cache_t(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32)] + [(n, ctypes.c_uint32) for n in (
+        "batch", "rows", "kv_heads", "head_dim", "page_size", "n_pages", "table_stride")] + [
+        ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3)]
+
+
+class es_cache_append_t(ctypes.Structure):
+    _fields_ = [("cache", es_paged_cache_t), ("in_dtype", ctypes.c_int32), ("heads", ctypes.c_uint32),
+                ("rotary_dim", ctypes.c_uint32), ("pairing", ctypes.c_int32), ("pos_offset", ctypes.c_int64),
+                ("n_positions", ctypes.c_uint64)] + [
+        (n, ctypes.c_int64 * 2) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")]
+
+
+class es_cache_append_args_t(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "q", "k", "v", "freqs", "q_out", "k_cache", "v_cache", "row_offsets", "lengths", "tables")]
+
+
+class es_paged_attention_t(ctypes.Structure):
+    _fields_ = [("cache", es_paged_cache_t), ("heads", ctypes.c_uint32), ("causal", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("prefix_len", ctypes.c_uint32),
+                ("q_stride", ctypes.c_int64 * 2), ("out_stride", ctypes.c_int64 * 2)]
+
+
+class es_paged_attention_args_t(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "q", "k_cache", "v_cache", "out", "lse", "row_offsets", "lengths", "tables", "prefix_pages")]
+
+
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libes_b200.so")
 
 # every symbol include/es_b200.h declares: name -> (restype, argtypes)
@@ -87,6 +116,10 @@ SYMBOLS = {
     "es_b200_flag_wait": (_i, [_vp, _vp, ctypes.c_uint32, _vp]),
     "es_b200_pull": (_i, [_vp, _vp, _vp, _u64, _vp]),
     "es_b200_launch_attention": (_i, [_vp, ctypes.POINTER(es_attention_t), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "es_b200_launch_cache_append": (_i, [_vp, _vp, _vp, _vp]),
+    "es_b200_paged_attention_workspace": (_i, [ctypes.POINTER(es_paged_attention_t), ctypes.POINTER(_u64)]),
+    "es_b200_launch_paged_attention": (_i, [_vp, _vp, _vp, _vp, _u64, _vp]),
+    "es_b200_launch_prefix_attention": (_i, [_vp, _vp, _vp, _vp, _u64, _vp]),
     "es_b200_kernel_info": (_i, [_vp, _u64, _cp, _i]),
     "es_b200_describe": (_i, [_desc_p, _i, _cp, _i]),
     "es_b200_touch_simplify": (_i, [_td_p, _i, _td_p, ctypes.POINTER(_i)]),
@@ -115,6 +148,10 @@ SYMBOLS = {
     "es_b200_load": (_i, [_vp, _vp, _i, _vp, _u64, _vp]),
     "es_b200_program_add_signal": (_i, [_vp, ctypes.POINTER(_vp), _i, _ip, _i, _ip]),
     "es_b200_program_add_attention": (_i, [_vp, ctypes.POINTER(es_attention_t), _vp, _vp, _vp, _vp, _vp, _ip, _i, _ip]),
+    "es_b200_program_add_cache_append": (_i, [_vp, ctypes.POINTER(es_cache_append_t),
+                                              ctypes.POINTER(es_cache_append_args_t), _ip, _i, _ip]),
+    "es_b200_program_add_paged_attention": (_i, [_vp, ctypes.POINTER(es_paged_attention_t),
+                                                 ctypes.POINTER(es_paged_attention_args_t), _ip, _i, _ip]),
     "es_b200_program_add_pull": (_i, [_vp, ctypes.POINTER(es_pull_item_t), _i, _ip, _i, _ip]),
     "es_b200_program_add_wait": (_i, [_vp, ctypes.POINTER(_vp), _i, _ip, _i, _ip]),
     "es_b200_program_finalize": (_i, [_vp, _i, ctypes.POINTER(_u64)]),

@@ -18,6 +18,7 @@
 #include "kernels.h"
 #include "attention.h"
 #include "nvtx_ranges.h"
+#include "paged.h"
 #include "exchange.h"
 #include "pdl.h"
 
@@ -571,6 +572,9 @@ int es_b200_device_status(es_b200_t* h, unsigned int* error_word)
         unsigned int tc = read_and_clear_tc_error();
         unsigned int at = read_and_clear_attention_error();
         if (!tc) tc = at;
+        unsigned int ap = read_and_clear_append_error();
+        unsigned int pg = read_and_clear_paged_error();
+        if (!tc) tc = ap ? ap : pg;
         unsigned int fl = read_and_clear_flag_error();
         unsigned int ex = read_and_clear_exchange_error();
         *error_word = tc | ((fl ? fl : ex) << 8);
@@ -637,6 +641,53 @@ int es_b200_launch_attention(es_b200_t* h, const es_attention_t* a, void* stream
         h->work_bytes[0] += attention_bytes(*a);
         h->work_flops += attention_flops(*a);
     });
+}
+
+int es_b200_launch_cache_append(es_b200_t* h, const es_cache_append_t* a, const es_cache_append_args_t* x, void* stream)
+{
+    return guarded([&] {
+        check_handle(h);
+        if (!a || !x) fail(ES_BAD_ARGUMENT, "cache append: null descriptor");
+        check_cache_append(*a, *x);
+        set_device(h);
+        nvtx_range_t range("cache_append");
+        h->counters[0] += launch_cache_append(*a, *x, (cudaStream_t)stream);
+        h->work_bytes[0] += cache_append_bytes(*a);
+    });
+}
+
+int es_b200_paged_attention_workspace(const es_paged_attention_t* a, uint64_t* bytes)
+{
+    return guarded([&] {
+        if (!a || !bytes) fail(ES_BAD_ARGUMENT, "paged attention: null pointer");
+        *bytes = paged_attention_workspace(*a);
+    });
+}
+
+static int launch_paged(es_b200_t* h, const es_paged_attention_t* a, const es_paged_attention_args_t* x, void* workspace,
+                        uint64_t workspace_bytes, void* stream, bool prefix)
+{
+    return guarded([&] {
+        check_handle(h);
+        if (!a || !x) fail(ES_BAD_ARGUMENT, "paged attention: null descriptor");
+        check_paged_attention(*a, *x, prefix);
+        set_device(h);
+        nvtx_range_t range(prefix ? "prefix_attention" : "paged_attention");
+        h->counters[0] += launch_paged_attention(*a, *x, workspace, workspace_bytes, (cudaStream_t)stream);
+        h->work_bytes[0] += paged_attention_bytes(*a);
+    });
+}
+
+int es_b200_launch_paged_attention(es_b200_t* h, const es_paged_attention_t* a, const es_paged_attention_args_t* x,
+                                   void* workspace, uint64_t workspace_bytes, void* stream)
+{
+    return launch_paged(h, a, x, workspace, workspace_bytes, stream, false);
+}
+
+int es_b200_launch_prefix_attention(es_b200_t* h, const es_paged_attention_t* a, const es_paged_attention_args_t* x,
+                                    void* workspace, uint64_t workspace_bytes, void* stream)
+{
+    return launch_paged(h, a, x, workspace, workspace_bytes, stream, true);
 }
 
 int es_b200_query_counters(es_b200_t* h, uint64_t launches[4])

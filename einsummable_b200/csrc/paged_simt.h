@@ -1,0 +1,220 @@
+// Paged attention without the tensor cores: f32, and f16 whose strides or head dim the other kernels do not
+// take.
+//
+// 8 lanes hold one key's head dim (4 elements at a time, 32 elements apart); a block's 16 such groups each
+// take every 16th key and keep running maxima, sums and results of their own for TR rows, so that nothing is
+// exchanged between groups until the segment ends.  The query rows stay in registers, multiplied by
+// scale * log2 e.  The next key and value are loaded before the current ones are used.  Bound: memory for up
+// to TR packed rows a key head; beyond that a key is read once per TR rows.
+#pragma once
+#include "paged_work.h"
+
+namespace es {
+namespace {
+
+constexpr int SIMT_BK = 64;
+
+// 4 elements of type T as f32; vec: one load, else the first n of them one by one
+template <typename T> __device__ __forceinline__ void load4(T const* p, float (&x)[4], bool vec, int n)
+{
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            float4 const t = *reinterpret_cast<float4 const*>(p);
+            x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+        } else {
+            uint2 const  t = *reinterpret_cast<uint2 const*>(p);
+            float2 const a = __half22float2(*reinterpret_cast<__half2 const*>(&t.x));
+            float2 const b = __half22float2(*reinterpret_cast<__half2 const*>(&t.y));
+            x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = i < n ? to_f32(p[i]) : 0.f;
+    }
+}
+
+template <typename T, int NCH, bool VEC> // NCH: chunks of 32 elements of the head dim
+__global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__ paged_params_t p)
+{
+    constexpr int TR = 16 / NCH, BK = SIMT_BK, NT = 128;
+    __shared__ sched_smem_t<NT> sched;
+    __shared__ float            so[4][TR][NCH * 32];
+    __shared__ float2           sml[4][TR];
+    ES_PDL_PROLOGUE();
+    int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, stream = threadIdx.x >> 3;
+    work_t    w;
+    find_work<TR, BK, NT>(p, w, sched);
+    bool split = false;
+    while (w.left) {
+        uint32_t const n_units = min(w.kt - w.j, w.left);
+        uint32_t const start = w.t * TR;
+        int const      count = (int)min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
+        float          q[TR][NCH][4], o[TR][NCH][4], m[TR], l[TR];
+        int            vis[TR], vis_max = 0;
+#pragma unroll
+        for (int r = 0; r < TR; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+            vis[r] = 0;
+            uint32_t const pr = start + r, tok = fdivide(pr, p.grp);
+            if (r < count) vis[r] = visible(p, w.s, (int)tok);
+            vis_max = max(vis_max, vis[r]);
+            T const* src = static_cast<T const*>(p.q) + (int64_t)(w.s.row0 + (int)tok) * p.q_stride[0] +
+                           (int64_t)(w.head * p.group + (pr - tok * p.group)) * p.q_stride[1];
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                uint32_t const e = c * 32 + l8 * 4;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[r][c][i] = o[r][c][i] = 0.f;
+                if (r < count && e < p.d) load4<T>(src + e, q[r][c], VEC, (int)(p.d - e));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[r][c][i] *= p.scale_log2;
+            }
+        }
+        int const key_end = (int)min((uint64_t)(w.j + n_units) * BK, (uint64_t)vis_max);
+        T const*  kb = static_cast<T const*>(p.k) + (int64_t)w.head * p.k_stride[2];
+        T const*  vb = static_cast<T const*>(p.v) + (int64_t)w.head * p.v_stride[2];
+        auto      load = [&](int key, float (&k)[NCH][4], float (&v)[NCH][4]) -> bool {
+            if (key >= key_end) return false;
+            uint32_t const pi = fdivide((uint32_t)key, p.page);
+            uint32_t const page = (uint32_t)w.s.table[pi];
+            if (page >= p.n_pages) {
+                report(p, PAGED_BAD_PAGE);
+                return false;
+            }
+            uint32_t const slot = (uint32_t)key - pi * p.page.d;
+            T const* const ks = kb + (int64_t)page * p.k_stride[0] + (int64_t)slot * p.k_stride[1];
+            T const* const vs = vb + (int64_t)page * p.v_stride[0] + (int64_t)slot * p.v_stride[1];
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                uint32_t const e = c * 32 + l8 * 4;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) k[c][i] = v[c][i] = 0.f;
+                if (e < p.d) {
+                    load4<T>(ks + e, k[c], VEC, (int)(p.d - e));
+                    load4<T>(vs + e, v[c], VEC, (int)(p.d - e));
+                }
+            }
+            return true;
+        };
+        float     k[NCH][4], v[NCH][4];
+        int const key0 = (int)(w.j * BK) + stream;
+        bool      have = load(key0, k, v);
+        // (every group of the warp makes the same number of rounds: the shuffles are the warp's)
+        int const rounds = key_end > (int)(w.j * BK) ? (key_end - (int)(w.j * BK) + 15) / 16 : 0;
+        for (int i = 0; i < rounds; ++i) {
+            int const key = key0 + i * 16;
+            float     kn[NCH][4], vn[NCH][4];
+            bool const next = i + 1 < rounds && load(key + 16, kn, vn);
+#pragma unroll
+            for (int r = 0; r < TR; ++r) {
+                float s = 0.f;
+#pragma unroll
+                for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s = fmaf(q[r][c][x], k[c][x], s);
+                s += __shfl_xor_sync(0xffffffffu, s, 4);
+                s += __shfl_xor_sync(0xffffffffu, s, 2);
+                s += __shfl_xor_sync(0xffffffffu, s, 1);
+                if (have && key < vis[r]) {
+                    if (s > m[r]) {
+                        float const a = exp2f(m[r] - s); // m = -inf: 0
+                        m[r] = s;
+                        l[r] *= a;
+#pragma unroll
+                        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) o[r][c][x] *= a;
+                    }
+                    float const e = exp2f(s - (m[r] == -INFINITY ? 0.f : m[r]));
+                    l[r] += e;
+#pragma unroll
+                    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[r][c][x] = fmaf(e, v[c][x], o[r][c][x]);
+                }
+            }
+            have = next;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    k[c][x] = kn[c][x];
+                    v[c][x] = vn[c][x];
+                }
+        }
+        // the warp's four groups
+#pragma unroll
+        for (int r = 0; r < TR; ++r) {
+#pragma unroll
+            for (int x = 8; x <= 16; x <<= 1) {
+                float const mo = __shfl_xor_sync(0xffffffffu, m[r], x), lo = __shfl_xor_sync(0xffffffffu, l[r], x);
+                float const mn = fmaxf(m[r], mo);
+                float const a = m[r] == -INFINITY ? (l[r] == 0.f ? 0.f : 1.f) : exp2f(m[r] - mn);
+                float const b = mo == -INFINITY ? (lo == 0.f ? 0.f : 1.f) : exp2f(mo - mn);
+                l[r] = l[r] * a + lo * b;
+#pragma unroll
+                for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float const oo = __shfl_xor_sync(0xffffffffu, o[r][c][i], x);
+                        o[r][c][i] = o[r][c][i] * a + oo * b;
+                    }
+                m[r] = mn;
+            }
+            if (lane < 8) {
+#pragma unroll
+                for (int c = 0; c < NCH; ++c)
+                    *reinterpret_cast<float4*>(&so[warp][r][c * 32 + l8 * 4]) = make_float4(o[r][c][0], o[r][c][1], o[r][c][2], o[r][c][3]);
+                if (l8 == 0) sml[warp][r] = make_float2(m[r], l[r]);
+            }
+        }
+        __syncthreads();
+        int const slot = segment_slot(w, n_units);
+        // the four warps' results; a thread 4 elements of a row
+        for (int x = threadIdx.x; x < count * NCH * 8; x += NT) {
+            int const      r = x / (NCH * 8);
+            uint32_t const e = (uint32_t)(x % (NCH * 8)) * 4;
+            float          top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (sml[i][r].y != 0.f) top = fmaxf(top, sml[i][r].x);
+            float sum[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float2 const ml = sml[i][r];
+                if (ml.y == 0.f) continue;
+                float const wgt = exp2f(ml.x - (top == -INFINITY ? 0.f : top));
+                float4 const a = *reinterpret_cast<float4 const*>(&so[i][r][e]);
+                ls = fmaf(ml.y, wgt, ls);
+                sum[0] = fmaf(a.x, wgt, sum[0]);
+                sum[1] = fmaf(a.y, wgt, sum[1]);
+                sum[2] = fmaf(a.z, wgt, sum[2]);
+                sum[3] = fmaf(a.w, wgt, sum[3]);
+            }
+            if (slot < 0) {
+                uint32_t const pr = start + r, tok = fdivide(pr, p.grp);
+                int const      row = w.s.row0 + (int)tok;
+                uint32_t const head = w.head * p.group + (pr - tok * p.group);
+                uint64_t const at = (uint64_t)row * p.heads + head;
+                finish_t const f = finish(top, ls, p.base_lse != nullptr, p.base_lse ? p.base_lse[at] : 0.f);
+                if (e < p.d) write_out<T, 4>(p, row, head, e, sum, f, VEC);
+                if (e == 0 && p.lse) p.lse[at] = f.lse;
+            } else {
+                uint64_t const at = (uint64_t)(2 * blockIdx.x + slot) * TR + r;
+                *reinterpret_cast<float4*>(p.part_out + at * p.part_d + e) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                if (e == 0) p.part_ml[at] = make_float2(top, ls);
+            }
+        }
+        __syncthreads();
+        if (slot == 1) {
+            split = true;
+            if (threadIdx.x == 0) write_meta<TR>(p, w, true);
+        }
+        next_item<TR, BK>(p, w, n_units);
+    }
+    if (!split && !p.direct && threadIdx.x == 0) write_meta<TR>(p, w, false);
+}
+
+} // namespace
+} // namespace es

@@ -1,0 +1,440 @@
+// The work of a paged attention call, how it is cut into equal shares, and how partial results are joined.
+//
+// An item is one (sequence, key / value head, tile of TR packed rows): packed row r of a sequence stands for
+// query head r % group of its token r / group, so that all heads that read the same keys share them.  An
+// item's keys are visited in tiles of BK; one (item, key tile) is a unit.  Lengths are known on the device
+// only, and differ: so every block counts all units (a scan over the batch), takes the same number of
+// consecutive units as every other block, and finds its first one.  An item inside one block's share is
+// finished there; one that crosses shares leaves an unnormalised partial result per share, at most two a
+// block (its first and its last item), which a second small kernel joins in order of the keys.  Nothing
+// depends on the order in which blocks run: the same call gives the same bits.
+#pragma once
+#include "paged_device.h"
+#include "pdl.h"
+
+namespace es {
+namespace {
+
+constexpr float LOG2_E = 1.4426950408889634f;
+constexpr float LN_2 = 0.6931471805599453f;
+
+struct paged_params_t {
+    void const*    q;
+    void const*    k;
+    void const*    v;
+    void*          out;         // rows of the cache's type, or (out_f32) the joined prefix in f32, dense
+    float*         lse;         // natural log; may be null
+    int32_t const* row_offsets; // may be null
+    int32_t const* lengths;
+    int32_t const* tables;
+    float const*   base_out;    // result over a prefix [rows, heads, d], merged in; may be null
+    float const*   base_lse;
+    float*         part_out;    // [blocks][2][TR][part_d]
+    float2*        part_ml;     // [blocks][2][TR]: maximum (log2 units), sum
+    int4*          meta;        // [blocks][2]
+    int64_t        q_stride[2], out_stride[2], k_stride[3], v_stride[3];
+    uint32_t       batch, rows, heads, kv_heads, group, d, part_d, n_pages, table_stride, capacity;
+    fastdiv_t      page, grp;
+    int32_t        causal;
+    int32_t        prefix_len;  // >= 0: all rows attend the one list of pages `tables`, of this many tokens
+    int32_t        direct;      // one block an item: nothing is split (one row a sequence)
+    uint32_t       packed_min, packed_max; // sequences with more than / at most so many packed rows
+    uint32_t       min_units;   // a block's share is at least this
+    float          scale_log2;  // scale * log2 e
+    int32_t        out_f32;
+    unsigned int*  error;
+};
+
+__device__ __forceinline__ void report(paged_params_t const& p, unsigned code)
+{
+    atomicCAS(p.error, 0u, code);
+}
+
+struct sequence_t {
+    int32_t        n;    // rows in this call (0: not this kernel's)
+    int32_t        len;  // tokens in the cache
+    int32_t        row0; // its first row
+    int32_t const* table;
+};
+
+__device__ __forceinline__ sequence_t get_sequence(paged_params_t const& p, uint32_t i)
+{
+    sequence_t s;
+    if (p.prefix_len >= 0) {
+        s.n = (int)p.rows;
+        if (p.row_offsets) {
+            s.n = p.row_offsets[p.batch];
+            if (s.n < 0 || s.n > (int)p.rows) {
+                report(p, PAGED_BAD_ROWS);
+                s.n = 0;
+            }
+        }
+        s.len = p.prefix_len;
+        s.row0 = 0;
+        s.table = p.tables;
+    } else {
+        s.len = p.lengths[i];
+        if (s.len < 0 || (uint32_t)s.len > p.capacity) {
+            report(p, PAGED_BAD_LENGTH);
+            s.len = 0;
+        }
+        s.row0 = (int)i;
+        s.n = 1;
+        if (p.row_offsets) {
+            int const a = p.row_offsets[i], b = p.row_offsets[i + 1];
+            s.row0 = a;
+            s.n = b - a;
+            if (a < 0 || b < a || b > (int)p.rows) {
+                report(p, PAGED_BAD_ROWS);
+                s.n = 0;
+            }
+        }
+        s.table = p.tables + (uint64_t)i * p.table_stride;
+    }
+    uint32_t const packed = (uint32_t)s.n * p.group; // < 2^31 (checked by the host)
+    if (packed <= p.packed_min || packed > p.packed_max) s.n = 0;
+    return s;
+}
+
+// keys that token `tok` of the sequence's rows may see
+__device__ __forceinline__ int visible(paged_params_t const& p, sequence_t const& s, int tok)
+{
+    return p.causal ? max(0, min(s.len, s.len - s.n + tok + 1)) : s.len;
+}
+
+// key tiles of the sequence's row tile t: those that its last token sees, one at least (it writes the result)
+template <int TR, int BK> __device__ __forceinline__ uint32_t tile_units(paged_params_t const& p, sequence_t const& s, uint32_t t)
+{
+    uint32_t const last = min((t + 1) * TR, (uint32_t)s.n * p.group) - 1;
+    uint32_t const keys = (uint32_t)visible(p, s, (int)fdivide(last, p.grp));
+    return max(1u, (keys + BK - 1) / BK);
+}
+template <int TR> __device__ __forceinline__ uint32_t row_tiles(paged_params_t const& p, sequence_t const& s)
+{
+    return ((uint32_t)s.n * p.group + TR - 1) / TR;
+}
+
+// Units of one head of the lane's sequence.  Causal parts of several tokens have row tiles of different
+// length: those are summed by the whole warp, one lane's sequence after the other.  All 32 lanes call.
+template <int TR, int BK> __device__ __forceinline__ uint64_t head_units(paged_params_t const& p, sequence_t const& s)
+{
+    uint64_t   u = 0;
+    bool const even = s.n <= 1 || !p.causal;
+    if (s.n > 0 && even) u = (uint64_t)row_tiles<TR>(p, s) * tile_units<TR, BK>(p, s, 0);
+    unsigned todo = __ballot_sync(0xffffffffu, s.n > 0 && !even);
+    int const lane = threadIdx.x & 31;
+    while (todo) {
+        int const  src = __ffs(todo) - 1;
+        sequence_t o;
+        o.n = __shfl_sync(0xffffffffu, s.n, src);
+        o.len = __shfl_sync(0xffffffffu, s.len, src);
+        uint32_t const rt = row_tiles<TR>(p, o);
+        uint64_t       sum = 0;
+        for (uint32_t t = lane; t < rt; t += 32) sum += tile_units<TR, BK>(p, o, t);
+#pragma unroll
+        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        if (lane == src) u = sum;
+        todo &= todo - 1;
+    }
+    return u;
+}
+
+// A block's place in the work
+struct work_t {
+    uint32_t   seq, head, t, rt;
+    uint32_t   j, kt;   // next key tile of the item, number of its key tiles
+    uint32_t   left;    // units of this block's share still to do
+    uint64_t   unit;    // number of the next unit
+    uint32_t   chunk;   // units a share
+    sequence_t s;
+};
+
+template <int NT> struct sched_smem_t {
+    uint64_t warp_sum[NT / 32];
+    uint64_t found_off;
+    uint32_t found_seq;
+};
+
+// All NT threads call; blockIdx.x is the block's number among gridDim.x.
+template <int TR, int BK, int NT>
+__device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sched_smem_t<NT>& sm)
+{
+    int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t const n_seq = p.prefix_len >= 0 ? 1u : p.batch;
+    w.left = 0;
+    w.j = 0;
+    w.unit = 0;
+    w.chunk = 0xffffffffu;
+    if (p.direct) {
+        // one row a sequence: item number = (sequence, head, row tile), nothing to count
+        w.rt = (p.group + TR - 1) / TR;
+        uint32_t const b = blockIdx.x;
+        w.t = b % w.rt;
+        w.head = (b / w.rt) % p.kv_heads;
+        w.seq = b / w.rt / p.kv_heads;
+        w.s = get_sequence(p, w.seq);
+        if (w.s.n == 0) return;
+        w.kt = tile_units<TR, BK>(p, w.s, w.t);
+        w.left = w.kt;
+        return;
+    }
+    uint64_t   mine = 0, u0 = 0;
+    for (uint32_t i0 = 0; i0 < n_seq; i0 += NT) {
+        sequence_t s;
+        s.n = 0;
+        s.len = 0;
+        if (i0 + threadIdx.x < n_seq) s = get_sequence(p, i0 + threadIdx.x);
+        u0 = head_units<TR, BK>(p, s) * p.kv_heads;
+        mine += u0;
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, x);
+    if (lane == 0) sm.warp_sum[warp] = mine;
+    __syncthreads();
+    uint64_t total = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) total += sm.warp_sum[i];
+    __syncthreads();
+    uint64_t const share = max((total + gridDim.x - 1) / gridDim.x, (uint64_t)p.min_units);
+    w.chunk = (uint32_t)min(share, (uint64_t)0xffffffffu);
+    uint64_t const lo = (uint64_t)blockIdx.x * w.chunk;
+    if (lo >= total) return; // (uniform)
+    w.unit = lo;
+    w.left = (uint32_t)min((uint64_t)w.chunk, total - lo);
+    // the sequence that holds unit `lo`
+    uint64_t base = 0;
+    for (uint32_t i0 = 0; i0 < n_seq; i0 += NT) {
+        uint64_t u = u0;
+        if (n_seq > NT) {
+            sequence_t s;
+            s.n = 0;
+            s.len = 0;
+            if (i0 + threadIdx.x < n_seq) s = get_sequence(p, i0 + threadIdx.x);
+            u = head_units<TR, BK>(p, s) * p.kv_heads;
+        }
+        uint64_t incl = u;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            uint64_t const o = __shfl_up_sync(0xffffffffu, incl, x);
+            if (lane >= x) incl += o;
+        }
+        if (lane == 31) sm.warp_sum[warp] = incl;
+        __syncthreads();
+        uint64_t before = base, all = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 32; ++i) {
+            if (i < warp) before += sm.warp_sum[i];
+            all += sm.warp_sum[i];
+        }
+        incl += before;
+        if (lo < incl && lo >= incl - u) {
+            sm.found_seq = i0 + threadIdx.x;
+            sm.found_off = lo - (incl - u);
+        }
+        base += all;
+        __syncthreads();
+        if (lo < base) break; // (uniform)
+    }
+    w.seq = sm.found_seq;
+    uint64_t off = sm.found_off;
+    w.s = get_sequence(p, w.seq);
+    uint64_t const per_head = head_units<TR, BK>(p, w.s); // every lane of every warp has the same sequence
+    w.head = (uint32_t)(off / per_head);
+    off -= w.head * per_head;
+    w.rt = row_tiles<TR>(p, w.s);
+    if (w.s.n <= 1 || !p.causal) {
+        w.kt = tile_units<TR, BK>(p, w.s, 0);
+        w.t = (uint32_t)(off / w.kt);
+        w.j = (uint32_t)(off - (uint64_t)w.t * w.kt);
+        return;
+    }
+    for (uint32_t t0 = 0;; t0 += 32) {
+        uint32_t const t = t0 + lane;
+        uint64_t const u = t < w.rt ? tile_units<TR, BK>(p, w.s, t) : 0;
+        uint64_t       incl = u;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            uint64_t const o = __shfl_up_sync(0xffffffffu, incl, x);
+            if (lane >= x) incl += o;
+        }
+        unsigned const hit = __ballot_sync(0xffffffffu, off < incl);
+        if (hit) {
+            int const src = __ffs(hit) - 1;
+            w.t = t0 + src;
+            w.kt = (uint32_t)__shfl_sync(0xffffffffu, u, src);
+            w.j = (uint32_t)(off - __shfl_sync(0xffffffffu, incl - u, src));
+            return;
+        }
+        off -= __shfl_sync(0xffffffffu, incl, 31);
+    }
+}
+
+// The next item, after `done` units of this one
+template <int TR, int BK> __device__ __forceinline__ void next_item(paged_params_t const& p, work_t& w, uint32_t done)
+{
+    w.left -= done;
+    w.unit += done;
+    w.j = 0;
+    if (w.left == 0) return;
+    if (++w.t == w.rt) {
+        w.t = 0;
+        if (++w.head == p.kv_heads) {
+            w.head = 0;
+            do { // (ends: units are left, so a sequence with some follows)
+                w.s = get_sequence(p, ++w.seq);
+            } while (w.s.n == 0);
+            w.rt = row_tiles<TR>(p, w.s);
+        }
+    }
+    w.kt = tile_units<TR, BK>(p, w.s, w.t);
+}
+
+// Where a segment's result goes: -1 finished here, 0 / 1 the block's first / last partial result
+__device__ __forceinline__ int segment_slot(work_t const& w, uint32_t n)
+{
+    if (w.j == 0 && n == w.kt) return -1;
+    return w.j == 0 ? 1 : 0;
+}
+
+// Every block says whether its last item goes on in the following blocks (thread 0)
+template <int TR>
+__device__ __forceinline__ void write_meta(paged_params_t const& p, work_t const& w, bool split)
+{
+    int4* m = p.meta + 2 * blockIdx.x;
+    if (!split) {
+        m[0] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    uint32_t const start = w.t * TR;
+    uint32_t const count = min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
+    uint64_t const last = w.unit + w.kt - 1; // unit numbers: w.unit is the item's first
+    m[0] = make_int4((int)count, w.s.row0, (int)start, (int)w.head);
+    m[1] = make_int4((int)(last / w.chunk), 0, 0, 0);
+}
+
+// The weights that turn an unnormalised sum (reference point m in log2 units, sum of exponentials l) and,
+// where there is one, the prefix's normalised result (natural log lse) into the result:
+// out = wa * sum + wb * prefix.  No key at all: both weights 0, lse -inf.
+struct finish_t {
+    float wa, wb, lse;
+};
+__device__ __forceinline__ finish_t finish(float m, float l, bool has_base, float base_lse)
+{
+    finish_t    f;
+    float const b2 = has_base ? base_lse * LOG2_E : -INFINITY;
+    float const top = fmaxf(l == 0.f ? -INFINITY : m, b2);
+    if (l == 0.f && b2 == -INFINITY) {
+        f.wa = f.wb = 0.f;
+        f.lse = -INFINITY;
+        return f;
+    }
+    float const a = l == 0.f ? 0.f : exp2f(m - top);
+    float const b = b2 == -INFINITY ? 0.f : exp2f(b2 - top);
+    float const total = fmaf(l, a, b);
+    f.wa = a / total;
+    f.wb = b / total;
+    f.lse = (top + log2f(total)) * LN_2;
+    return f;
+}
+
+// W consecutive elements (4 or 2 or 1) of a finished row
+template <typename T, int W>
+__device__ __forceinline__ void write_out(paged_params_t const& p, int row, uint32_t head, uint32_t e, float const (&o)[W],
+                                          finish_t const& f, bool aligned)
+{
+    float r[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) r[i] = f.wa == 0.f ? 0.f : o[i] * f.wa; // a weight of 0: the sum may be anything
+    if (p.base_out && f.wb != 0.f) {
+        float const* b = p.base_out + ((uint64_t)row * p.heads + head) * p.d + e;
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            if (e + i < p.d) r[i] = fmaf(b[i], f.wb, r[i]);
+    }
+    if (p.out_f32) {
+        float* d = static_cast<float*>(p.out) + ((uint64_t)row * p.heads + head) * p.d + e;
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            if (e + i < p.d) d[i] = r[i];
+        return;
+    }
+    T* d = static_cast<T*>(p.out) + (int64_t)row * p.out_stride[0] + (int64_t)head * p.out_stride[1] + e;
+    if (aligned && e + W <= p.d) {
+        if constexpr (sizeof(T) == 4) {
+            if constexpr (W == 4) *reinterpret_cast<float4*>(d) = make_float4(r[0], r[1], r[2], r[3]);
+            else if constexpr (W == 2) *reinterpret_cast<float2*>(d) = make_float2(r[0], r[1]);
+            else d[0] = r[0];
+        } else {
+            if constexpr (W == 4) {
+                __half2 const a = __floats2half2_rn(r[0], r[1]), b = __floats2half2_rn(r[2], r[3]);
+                *reinterpret_cast<uint2*>(d) = make_uint2(*reinterpret_cast<uint32_t const*>(&a), *reinterpret_cast<uint32_t const*>(&b));
+            } else if constexpr (W == 2) {
+                *reinterpret_cast<__half2*>(d) = __floats2half2_rn(r[0], r[1]);
+            } else {
+                from_f32(d[0], r[0]);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+        if (e + i < p.d) from_f32(d[i], r[i]);
+}
+
+// Joins the partial results of the items that crossed shares.  Block x: the item that starts last in share x
+// (if it goes on behind it); a warp a row; lanes over the head dim.
+template <typename T, int TR>
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ paged_params_t p, int aligned)
+{
+    ES_PDL_PROLOGUE();
+    int4 const     m0 = p.meta[2 * blockIdx.x];
+    uint32_t const r = blockIdx.y * 4 + (threadIdx.x >> 5);
+    if (r >= (uint32_t)m0.x) return;
+    int const      last = p.meta[2 * blockIdx.x + 1].x;
+    uint32_t const lane = threadIdx.x & 31;
+    int const      first = (int)blockIdx.x, n = last - first + 1;
+    // part i lies in share first + i: its last slot for i = 0, the first slot of the others
+    auto slot = [&](int i) { return (uint64_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * TR + r; };
+    float top = -INFINITY;
+    for (int i = (int)lane; i < n; i += 32) {
+        float2 const ml = p.part_ml[slot(i)];
+        if (ml.y != 0.f) top = fmaxf(top, ml.x);
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    float o[2][4] = {}, l = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        float2 const ml = p.part_ml[slot(i)];
+        if (ml.y == 0.f) continue; // no key
+        float const  wgt = exp2f(ml.x - top);
+        float const* src = p.part_out + slot(i) * p.part_d;
+        l = fmaf(ml.y, wgt, l);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            uint32_t const e = c * 128 + lane * 4;
+            if (e < p.part_d) {
+                float4 const x = *reinterpret_cast<float4 const*>(src + e);
+                o[c][0] = fmaf(x.x, wgt, o[c][0]);
+                o[c][1] = fmaf(x.y, wgt, o[c][1]);
+                o[c][2] = fmaf(x.z, wgt, o[c][2]);
+                o[c][3] = fmaf(x.w, wgt, o[c][3]);
+            }
+        }
+    }
+    uint32_t const pr = (uint32_t)m0.z + r;
+    uint32_t const tok = fdivide(pr, p.grp);
+    int const      row = m0.y + (int)tok;
+    uint32_t const head = (uint32_t)m0.w * p.group + (pr - tok * p.group);
+    uint64_t const at = (uint64_t)row * p.heads + head;
+    finish_t const f = finish(top, l, p.base_lse != nullptr, p.base_lse ? p.base_lse[at] : 0.f);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        uint32_t const e = c * 128 + lane * 4;
+        if (e < p.d) write_out<T, 4>(p, row, head, e, o[c], f, aligned != 0);
+    }
+    if (p.lse && lane == 0) p.lse[at] = f.lse;
+}
+
+} // namespace
+} // namespace es

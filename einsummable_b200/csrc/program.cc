@@ -38,6 +38,7 @@
 #include "handle.h"
 #include "kernels.h"
 #include "nvtx_ranges.h"
+#include "paged.h"
 #include "pdl.h"
 
 namespace {
@@ -56,12 +57,14 @@ enum op_kind_t {
     OP_TOUCH_BATCH = 8,
     OP_EVICT = 9,
     OP_LOAD = 10,
-    OP_ATTENTION = 11
+    OP_ATTENTION = 11,
+    OP_CACHE_APPEND = 12,
+    OP_PAGED_ATTENTION = 13
 };
 
 char const* const OP_NAMES[] = {"einsummable", "touch", "fill_constant", "fill_lowertri", "copy",
                                 "signal",      "pull",  "wait",          "touch_batch",   "evict",
-                                "load",        "attention"};
+                                "load",        "attention", "cache_append", "paged_attention"};
 
 struct op_t {
     int              kind = 0;
@@ -86,6 +89,10 @@ struct op_t {
     std::vector<pull_item_t> pulls;      // pull
     std::vector<touch_args_t> batch;     // touch batch (one dtype, one width)
     es_attention_t           attn;
+    es_cache_append_t        append;
+    es_cache_append_args_t   append_args;
+    es_paged_attention_t     paged;
+    es_paged_attention_args_t paged_args;
     uint64_t                 batch_slots = 0;
     // device-side descriptor arrays (finalize)
     uint64_t                 dev_off = 0, dev_off2 = 0;
@@ -232,7 +239,7 @@ void schedule(es_b200_program* p, int max_lanes)
     p->lane_ws_off.assign(p->n_lanes, 0);
     std::vector<uint64_t> need_ws(p->n_lanes, 0);
     for (auto const& op : ops)
-        if (op.kind == OP_EINSUMMABLE) need_ws[op.lane] = std::max(need_ws[op.lane], op.ws_need);
+        if (op.kind == OP_EINSUMMABLE || op.kind == OP_PAGED_ATTENTION) need_ws[op.lane] = std::max(need_ws[op.lane], op.ws_need);
     uint64_t off = 0;
     for (int l = 0; l != p->n_lanes; ++l) {
         p->lane_ws_off[l] = off;
@@ -344,6 +351,15 @@ void launch_op(es_b200_program* p, op_t const& op, cudaStream_t s)
             h->counters[0] += 1;
             h->work_bytes[0] += op.work_bytes;
             h->work_flops += attention_flops(op.attn);
+            break;
+        case OP_CACHE_APPEND:
+            h->counters[0] += launch_cache_append(op.append, op.append_args, s);
+            h->work_bytes[0] += op.work_bytes;
+            break;
+        case OP_PAGED_ATTENTION:
+            h->counters[0] += launch_paged_attention(op.paged, op.paged_args, p->ws_base + p->lane_ws_off[op.lane],
+                                                     round_up(op.ws_need, 256), s);
+            h->work_bytes[0] += op.work_bytes;
             break;
         case OP_COPY:
             launch_pull_copy(op.src, op.out, op.bytes, s);
@@ -656,6 +672,40 @@ int es_b200_program_add_attention(es_b200_program_t* p, const es_attention_t* a,
         op.out = out;
         op.inns = {q, k, v, mask};
         op.work_bytes = attention_bytes(*a);
+        add_op(p, std::move(op), deps, n_deps, op_index);
+    });
+}
+
+int es_b200_program_add_cache_append(es_b200_program_t* p, const es_cache_append_t* a, const es_cache_append_args_t* x,
+                                     const int* deps, int n_deps, int* op_index)
+{
+    return guarded([&] {
+        check_program(p, false);
+        if (!a || !x) fail(ES_BAD_ARGUMENT, "program cache append: null descriptor");
+        check_cache_append(*a, *x);
+        op_t op;
+        op.kind = OP_CACHE_APPEND;
+        op.append = *a;
+        op.append_args = *x;
+        op.work_bytes = cache_append_bytes(*a);
+        add_op(p, std::move(op), deps, n_deps, op_index);
+    });
+}
+
+int es_b200_program_add_paged_attention(es_b200_program_t* p, const es_paged_attention_t* a,
+                                        const es_paged_attention_args_t* x,
+                                        const int* deps, int n_deps, int* op_index)
+{
+    return guarded([&] {
+        check_program(p, false);
+        if (!a || !x) fail(ES_BAD_ARGUMENT, "program paged attention: null descriptor");
+        check_paged_attention(*a, *x, a->prefix_len > 0);
+        op_t op;
+        op.kind = OP_PAGED_ATTENTION;
+        op.paged = *a;
+        op.paged_args = *x;
+        op.ws_need = paged_attention_workspace(*a);
+        op.work_bytes = paged_attention_bytes(*a);
         add_op(p, std::move(op), deps, n_deps, op_index);
     });
 }

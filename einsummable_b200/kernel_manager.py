@@ -18,6 +18,9 @@ from .einsummable import CASTABLE_CODE, einsummable_t, fill_t, touch_t
 from .scalarop import DTYPE_CODE
 
 
+_byref = ctypes.byref
+
+
 def _ptr(x):
     if x is None:
         return None
@@ -198,6 +201,41 @@ class kernel_manager_t:
         _lib.check(self._lib.es_b200_launch_attention(
             self._h, ctypes.byref(c), _stream(stream), _ptr(out), _ptr(q), _ptr(k), _ptr(v),
             _ptr(mask) if mask is not None else None))
+
+    def cache_append(self, desc, stream, k_cache, v_cache, k, v, lengths, tables, row_offsets=None, freqs=None, q=None,
+                     q_out=None):
+        """The step's new keys, rotated by their positions, and values into the pages of the cache; its queries
+        rotated into q_out.  `desc` is a cache_append_t (einsummable_b200.paged); lengths [batch] count the new
+        tokens already, tables [batch, table_stride] and row_offsets [batch + 1] (None: one row a sequence) are
+        int32 on the device, freqs the complex64 table [n_positions, rotary_dim / 2]."""
+        x = _lib.es_cache_append_args_t(_ptr(q), _ptr(k), _ptr(v), _ptr(freqs), _ptr(q_out), _ptr(k_cache), _ptr(v_cache),
+                                        _ptr(row_offsets), _ptr(lengths), _ptr(tables))
+        _lib.check(self._lib.es_b200_launch_cache_append(self._h, _byref(desc.c), _byref(x), _stream(stream)))
+
+    def paged_attention_workspace(self, desc):
+        """Bytes of workspace that an attention over the paged cache needs (a paged_attention_t)."""
+        n = ctypes.c_uint64(0)
+        _lib.check(self._lib.es_b200_paged_attention_workspace(ctypes.byref(desc.c), ctypes.byref(n)))
+        return n.value
+
+    def paged_attention(self, desc, stream, out, q, k_cache, v_cache, lengths, tables, row_offsets=None, lse=None,
+                        workspace=None):
+        """Attention of the step's queries to their own sequences' keys in the cache; lse [rows, heads] f32 gets
+        the logarithm of the sums of exponentials.  `desc` is a paged_attention_t (einsummable_b200.paged), the
+        arrays as for cache_append, workspace = (device memory, bytes)."""
+        x = _lib.es_paged_attention_args_t(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(lse), _ptr(row_offsets),
+                                           _ptr(lengths), _ptr(tables), None)
+        ws, n = (None, 0) if workspace is None else (_ptr(workspace[0]), int(workspace[1]))
+        _lib.check(self._lib.es_b200_launch_paged_attention(self._h, _byref(desc.c), _byref(x), ws, n, _stream(stream)))
+
+    def prefix_attention(self, desc, stream, out, q, k_cache, v_cache, prefix_pages, lengths, tables, row_offsets=None,
+                         lse=None, workspace=None):
+        """The same behind a prefix that all sequences share: its desc.prefix_len tokens lie in the pages
+        prefix_pages (int32 on the device) and are read once for the whole batch."""
+        x = _lib.es_paged_attention_args_t(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(lse), _ptr(row_offsets),
+                                           _ptr(lengths), _ptr(tables), _ptr(prefix_pages))
+        ws, n = (None, 0) if workspace is None else (_ptr(workspace[0]), int(workspace[1]))
+        _lib.check(self._lib.es_b200_launch_prefix_attention(self._h, _byref(desc.c), _byref(x), ws, n, _stream(stream)))
 
     def rowsum_f32_noalloc(self, stream, out, inn, rows, cols):
         """out[a] = sum_b inn[a,b] for f32 without any device allocation: the

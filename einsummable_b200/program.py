@@ -119,6 +119,29 @@ class program_t:
             _ptr(mask) if mask is not None else None, d, nd, ctypes.byref(idx)))
         return self._added(idx)
 
+    def add_cache_append(self, desc, k_cache, v_cache, k, v, lengths, tables, row_offsets=None, freqs=None, q=None,
+                         q_out=None, deps=()):
+        """kernel_manager_t.cache_append as one op (desc: cache_append_t)."""
+        x = _lib.es_cache_append_args_t(*[_ptr(t) for t in (q, k, v, freqs, q_out, k_cache, v_cache, row_offsets, lengths,
+                                                            tables)])
+        d, nd = _deps(deps)
+        idx = ctypes.c_int(-1)
+        _lib.check(self._lib.es_b200_program_add_cache_append(self._p, ctypes.byref(desc.c), ctypes.byref(x), d, nd,
+                                                              ctypes.byref(idx)))
+        return self._added(idx)
+
+    def add_paged_attention(self, desc, out, q, k_cache, v_cache, lengths, tables, row_offsets=None, lse=None,
+                            prefix_pages=None, deps=()):
+        """kernel_manager_t.paged_attention -- or, with desc.prefix_len > 0, prefix_attention -- as one op
+        (desc: paged_attention_t)."""
+        x = _lib.es_paged_attention_args_t(*[_ptr(t) for t in (q, k_cache, v_cache, out, lse, row_offsets, lengths, tables,
+                                                               prefix_pages)])
+        d, nd = _deps(deps)
+        idx = ctypes.c_int(-1)
+        _lib.check(self._lib.es_b200_program_add_paged_attention(self._p, ctypes.byref(desc.c), ctypes.byref(x), d, nd,
+                                                                 ctypes.byref(idx)))
+        return self._added(idx)
+
     def add_copy(self, src, dst, nbytes, deps=()):
         d, nd = _deps(deps)
         idx = ctypes.c_int(-1)

@@ -258,6 +258,110 @@ typedef struct {
 int es_b200_launch_attention(es_b200_t* h, const es_attention_t* a, void* stream, void* out,
                              const void* q, const void* k, const void* v, const void* mask);
 
+/* ---- Generating tokens: a paged cache of keys and values -----------------------------------------
+ * The reference keeps a cache per layer and concatenates every new token's keys and values to it
+ * (attention_t::forward, llama/modules.cc:285-383), which copies the whole cache once a token.  Here the cache of one layer is a set of fixed pages; a sequence is a
+ * list of pages (a row of `tables`) and a length, and may grow without anything being moved.
+ *
+ * The batch of one step, given to every call of the step (arrays in device memory, read when the kernels
+ * run, so that a captured step can be replayed after they changed):
+ *   lengths[batch]             tokens of the sequence in the cache, the new ones of this step included
+ *   tables[batch][table_stride] pages of the sequence, in order; entries behind its last page are not read
+ *   row_offsets[batch + 1]     row r of the step's tensors belongs to sequence i when row_offsets[i] <= r <
+ *                              row_offsets[i + 1] (ascending from 0); rows from row_offsets[batch] on are
+ *                              padding and are left as they are.  NULL: one row a sequence, rows == batch.
+ * Row r of sequence i is its token number p = lengths[i] - (row_offsets[i + 1] - row_offsets[i]) + (r -
+ * row_offsets[i]).  A row with p < 0 has no place in the cache (an unused place of the batch: length 0).
+ * Page size, strides and page order are free: token p lies in slot p % page_size of page
+ * tables[i][p / page_size], at element page * stride[0] + slot * stride[1] + head * stride[2], the head
+ * dim contiguous.  What lies in the pages behind a sequence's last token is never used.
+ *
+ * What the arrays hold is checked on the device: a page number outside [0, n_pages) (0x21), a length
+ * outside [0, table_stride * page_size] (0x22), row offsets that fall, go negative or pass `rows` (0x23), or
+ * a position outside the table of angles (0x24) skips the access, leaves the rest of the batch right and
+ * is reported by es_b200_device_status. */
+typedef struct {
+    int32_t  dtype;        /* ES_F16 or ES_F32 */
+    uint32_t batch;        /* sequences */
+    uint32_t rows;         /* rows of the step's tensors */
+    uint32_t kv_heads, head_dim;
+    uint32_t page_size;    /* tokens a page */
+    uint32_t n_pages;
+    uint32_t table_stride; /* pages a row of tables */
+    int64_t  k_stride[3];  /* elements: page, slot, head */
+    int64_t  v_stride[3];
+} es_paged_cache_t;
+
+/* The step's keys, rotated by their positions, and values into the cache, and its queries rotated: with
+ * f = freqs[p + pos_offset], the complex table [n_positions, rotary_dim / 2] of the reference's models
+ * (its full_freqs_cis), pair j of a query or key becomes (x + i y) f[j]; its members are elements 2j and
+ * 2j + 1 (ES_ROPE_ADJACENT, the reference's) or j and j + rotary_dim / 2 (ES_ROPE_HALVES).  Elements from
+ * rotary_dim on are copied.  Computed in f32, rounded once to the cache's type.  heads = 0: no queries;
+ * rotary_dim = 0: no rotation (freqs may be NULL).  q_out may be q itself where types and strides agree;
+ * it may not overlap it otherwise.  When two rows name the same slot, which of them it holds is open. */
+typedef enum { ES_ROPE_ADJACENT = 0, ES_ROPE_HALVES = 1 } es_rope_pairing_t;
+typedef struct {
+    es_paged_cache_t cache;
+    int32_t  in_dtype;   /* of q, k, v: ES_F16 or ES_F32; q_out has the cache's */
+    uint32_t heads;      /* of the queries */
+    uint32_t rotary_dim; /* even, at most head_dim */
+    int32_t  pairing;    /* es_rope_pairing_t */
+    int64_t  pos_offset; /* >= 0: e.g. the length of a prefix that lies in front of every sequence */
+    uint64_t n_positions;
+    int64_t  q_stride[2], k_stride[2], v_stride[2], q_out_stride[2]; /* elements: row, head */
+} es_cache_append_t;
+typedef struct {
+    const void*    q;
+    const void*    k;
+    const void*    v;
+    const float*   freqs; /* real and imaginary part of each factor */
+    void*          q_out;
+    void*          k_cache;
+    void*          v_cache;
+    const int32_t* row_offsets; /* or NULL */
+    const int32_t* lengths;
+    const int32_t* tables;
+} es_cache_append_args_t;
+int es_b200_launch_cache_append(es_b200_t* h, const es_cache_append_t* a, const es_cache_append_args_t* x, void* stream);
+
+/* Attention of the step's queries to their own sequences' keys in the cache:
+ *   s_j = scale * q . k_j    for j <= p (causal) or every token of the sequence (not causal)
+ *   out = sum_j exp(s_j - lse) v_j,   lse = log sum_j exp(s_j)
+ * A row that sees no key gets out = 0 and lse = -inf.  Query head h reads key / value head
+ * h / (heads / kv_heads).  Any head dim up to 256, any strides; f16 with a head dim that is a multiple of
+ * 8 up to 128, strides that are multiples of 8 and 16-byte aligned pointers runs on the tensor cores.
+ * f32 accumulation and statistics; with f16 on the tensor cores the probabilities are rounded to f16 for
+ * the product with the values.  Inside one sequence a masked token's values must be finite (0 * inf).
+ * prefix_len tokens, the same for all sequences and listed by prefix_pages, can lie in front of every
+ * sequence's own (es_b200_launch_prefix_attention): every row sees all of them, and they are read once
+ * for the whole batch.  lengths and tables then count a sequence's own tokens only.
+ * The workspace (es_b200_paged_attention_workspace; 16-byte aligned, contents irrelevant before and
+ * after) may be shared by calls that do not overlap in time. */
+typedef struct {
+    es_paged_cache_t cache; /* dtype also of q and out */
+    uint32_t heads;         /* a multiple of cache.kv_heads */
+    int32_t  causal;
+    float    scale;
+    uint32_t prefix_len;
+    int64_t  q_stride[2], out_stride[2]; /* elements: row, head */
+} es_paged_attention_t;
+typedef struct {
+    const void*    q;
+    const void*    k_cache;
+    const void*    v_cache;
+    void*          out;
+    float*         lse;          /* [rows, heads], or NULL */
+    const int32_t* row_offsets;  /* or NULL */
+    const int32_t* lengths;
+    const int32_t* tables;
+    const int32_t* prefix_pages; /* [ceil(prefix_len / page_size)]; NULL when prefix_len is 0 */
+} es_paged_attention_args_t;
+int es_b200_paged_attention_workspace(const es_paged_attention_t* a, uint64_t* bytes);
+int es_b200_launch_paged_attention(es_b200_t* h, const es_paged_attention_t* a, const es_paged_attention_args_t* x,
+                                   void* workspace, uint64_t workspace_bytes, void* stream);
+int es_b200_launch_prefix_attention(es_b200_t* h, const es_paged_attention_t* a, const es_paged_attention_args_t* x,
+                                    void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* Introspection: "kind|merged str|vector width|..." of a built kernel. */
 int es_b200_kernel_info(es_b200_t* h, uint64_t kernel_id, char* buf, int buf_len);
 
@@ -304,7 +408,8 @@ int es_b200_rowsum_f32_noalloc(es_b200_t*   h,
  * tensor-core kernels: 0 = fine; nonzero = a bounded wait inside a kernel gave
  * up (1 producer, 2/3 MMA issuer, 4 epilogue) and that launch's output is not
  * valid; 0x11..0x16 = the same inside the attention kernel (Q copy, K copy, scores, P tile,
- * V copy, P V).  The reference has no counterpart: its library kernels cannot report. */
+ * V copy, P V), 0x21..0x24 = what a paged-cache kernel found in its arrays, 0x31..0x38 = a wait inside
+ * the paged attention kernel.  The reference has no counterpart: its library kernels cannot report. */
 int es_b200_device_status(es_b200_t* h, unsigned int* error_word);
 
 /* Clock trace of the tensor-core contraction kernel (trace builds only: the library compiled
@@ -411,6 +516,14 @@ int es_b200_program_add_load(es_b200_program_t* p, const void* host_src, void* d
 int es_b200_program_add_attention(es_b200_program_t* p, const es_attention_t* a, void* out,
                                   const void* q, const void* k, const void* v, const void* mask,
                                   const int* deps, int n_deps, int* op_index);
+/* The step of a paged cache as ops of the program; the workspace comes from
+ * es_b200_program_set_workspace.  add_paged_attention is also the attention behind a prefix
+ * (a->prefix_len > 0). */
+int es_b200_program_add_cache_append(es_b200_program_t* p, const es_cache_append_t* a, const es_cache_append_args_t* x,
+                                     const int* deps, int n_deps, int* op_index);
+int es_b200_program_add_paged_attention(es_b200_program_t* p, const es_paged_attention_t* a,
+                                        const es_paged_attention_args_t* x,
+                                        const int* deps, int n_deps, int* op_index);
 int es_b200_program_add_signal(es_b200_program_t* p, void* const* flags, int n,
                                const int* deps, int n_deps, int* op_index);
 int es_b200_program_add_pull(es_b200_program_t* p, const es_pull_item_t* items, int n,
