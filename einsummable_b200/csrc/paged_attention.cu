@@ -7,11 +7,11 @@
 // into an f32 result and its lse; the sequences' own keys follow, and the two are weighed by exp(lse) where a
 // row is finished.
 #include <algorithm>
-#include <cmath>
 #include <cstring>
 #include <string>
 
 #include "paged.h"
+#include "paged_mma.h"
 #include "paged_simt.h"
 #include "paged_work.h"
 
@@ -22,6 +22,7 @@ namespace {
 __device__ unsigned int g_paged_error;
 
 constexpr uint32_t SIMT_BLOCKS = 2 * SM_COUNT;
+constexpr uint32_t MMA_BLOCKS = 2 * SM_COUNT, MMA_WORKERS = MMA_BLOCKS * MMA_WARPS, MMA_MAX_TR = 32;
 
 uint64_t align256(uint64_t x)
 {
@@ -36,15 +37,20 @@ layout_t layout(es_paged_attention_t const& a)
 {
     es_paged_cache_t const& c = a.cache;
     layout_t                l;
-    uint64_t const          blocks = SIMT_BLOCKS;
-    uint64_t const          part = 2 * blocks * 16 * 32; // slots x rows x head dim
-    uint64_t                at = 0;
+    // of every kernel that the pointers may make the call choose: workers x 2 slots x rows (x head dim)
+    uint64_t part = 2ull * SIMT_BLOCKS * 16 * 32, ml = 2ull * SIMT_BLOCKS * 8, meta = SIMT_BLOCKS;
+    if (c.dtype == ES_F16 && c.head_dim <= 128) {
+        part = std::max<uint64_t>(part, 2ull * MMA_WORKERS * MMA_MAX_TR * (c.head_dim <= 64 ? 64 : 128));
+        ml = std::max<uint64_t>(ml, 2ull * MMA_WORKERS * MMA_MAX_TR);
+        meta = std::max<uint64_t>(meta, MMA_WORKERS);
+    }
+    uint64_t at = 0;
     l.part_out = at;
     at += align256(part * 4);
     l.part_ml = at;
-    at += align256(2 * blocks * 8 * 8);
+    at += align256(ml * 8);
     l.meta = at;
-    at += align256(2 * blocks * 16);
+    at += align256(meta * 2 * 16);
     l.base_out = at;
     if (a.prefix_len) at += align256((uint64_t)c.rows * a.heads * c.head_dim * 4);
     l.base_lse = at;
@@ -72,7 +78,8 @@ bool aligned16(es_paged_attention_t const& a, es_paged_attention_args_t const& x
     for (int i = 0; i != 3; ++i) el |= (uint64_t)c.k_stride[i] | (uint64_t)c.v_stride[i];
     uintptr_t const bits = reinterpret_cast<uintptr_t>(x.q) | reinterpret_cast<uintptr_t>(x.out) |
                            reinterpret_cast<uintptr_t>(x.k_cache) | reinterpret_cast<uintptr_t>(x.v_cache);
-    return (el % per) == 0 && (bits & 15) == 0;
+    // (the tensor-core kernels step through a page in 32 bits of bytes)
+    return (el % per) == 0 && (bits & 15) == 0 && c.k_stride[1] < (1 << 26) && c.v_stride[1] < (1 << 26);
 }
 
 template <typename T> int launch_simt(paged_params_t& p, bool vec, cudaStream_t stream)
@@ -83,19 +90,56 @@ template <typename T> int launch_simt(paged_params_t& p, bool vec, cudaStream_t 
     // Direct: with at most 8 key tiles an item, one block an item and no join -- a join costs as much as
     // about 8 tiles take
     p.direct = !p.row_offsets && p.prefix_len < 0 && p.capacity <= 8 * SIMT_BK;
-    uint64_t const items = (uint64_t)p.batch * p.kv_heads * ((p.group + tr - 1) / tr);
-    if (items > 0x7fffffffull) p.direct = 0;
-    uint32_t const grid = p.direct ? (uint32_t)items : SIMT_BLOCKS;
-    auto           go = [&](auto kernel) { launch_k(kernel, dim3(grid), dim3(128), 0, stream, p); };
+    if (p.batch > 65535) p.direct = 0;
+    uint32_t const grid = p.direct ? p.kv_heads * ((p.group + tr - 1) / tr) : SIMT_BLOCKS;
+    auto           go = [&](auto kernel) { launch_k(kernel, dim3(grid, p.direct ? p.batch : 1), dim3(128), 0, stream, p); };
     if (nch == 2) vec ? go(paged_simt_kernel<T, 2, true>) : go(paged_simt_kernel<T, 2, false>);
     else if (nch == 4) vec ? go(paged_simt_kernel<T, 4, true>) : go(paged_simt_kernel<T, 4, false>);
     else vec ? go(paged_simt_kernel<T, 8, true>) : go(paged_simt_kernel<T, 8, false>);
     if (p.direct) return 1;
     pdl_scope_t scope(true);
-    auto        join = [&](auto kernel) { launch_k(kernel, dim3(grid, (tr + 3) / 4), dim3(128), 0, stream, p, vec ? 1 : 0); };
-    if (nch == 2) join(paged_join_kernel<T, 8>);
-    else if (nch == 4) join(paged_join_kernel<T, 4>);
-    else join(paged_join_kernel<T, 2>);
+    auto        join = [&](auto kernel) { launch_k(kernel, dim3(grid), dim3(256), 0, stream, p, vec ? 1 : 0); };
+    if (nch == 2) join(paged_join_kernel<T, 8, 1>);
+    else if (nch == 4) join(paged_join_kernel<T, 4, 1>);
+    else join(paged_join_kernel<T, 2, 2>);
+    return 2;
+}
+
+// Kernels with more shared memory than 48 KB say so once per device
+template <typename K> void allow_smem(K kernel, uint32_t bytes, bool (&done)[64])
+{
+    int dev = 0;
+    ES_CUDA_CHECK(cudaGetDevice(&dev));
+    if (done[dev & 63]) return;
+    ES_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    done[dev & 63] = true;
+}
+
+template <int DPAD, int NT, bool PAGE16> void launch_mma_as(paged_params_t const& p, dim3 grid, uint32_t q_rows, cudaStream_t stream)
+{
+    static bool done[64] = {};
+    allow_smem(paged_mma_kernel<DPAD, NT, PAGE16>, MMA_WARPS * mma_warp_bytes<DPAD>(8 * NT), done);
+    launch_k(paged_mma_kernel<DPAD, NT, PAGE16>, grid, dim3(MMA_WARPS * 32), MMA_WARPS * mma_warp_bytes<DPAD>(q_rows), stream, p, q_rows);
+}
+
+template <int NT> int launch_mma(paged_params_t& p, cudaStream_t stream)
+{
+    constexpr uint32_t TR = 8 * NT;
+    bool const         page16 = p.page.d % MMA_BK == 0;
+    p.part_d = p.d <= 64 ? 64 : 128;
+    // Direct: with at most 16 key tiles an item, one warp an item and no join
+    p.direct = !p.row_offsets && p.prefix_len < 0 && p.capacity <= 16 * MMA_BK;
+    p.min_units = 4;
+    if (p.batch > 65535) p.direct = 0;
+    uint32_t const items = p.kv_heads * ((p.group + TR - 1) / TR); // of a sequence
+    dim3 const     grid(p.direct ? (items + MMA_WARPS - 1) / MMA_WARPS : MMA_BLOCKS, p.direct ? p.batch : 1);
+    // rows of a query tile: the packed rows of one token, or of all there are
+    uint32_t const q_rows = std::min<uint32_t>(TR, !p.row_offsets && p.prefix_len < 0 ? p.group : p.rows * p.group);
+    if (p.part_d == 64) page16 ? launch_mma_as<64, NT, true>(p, grid, q_rows, stream) : launch_mma_as<64, NT, false>(p, grid, q_rows, stream);
+    else page16 ? launch_mma_as<128, NT, true>(p, grid, q_rows, stream) : launch_mma_as<128, NT, false>(p, grid, q_rows, stream);
+    if (p.direct) return 1;
+    pdl_scope_t scope(true);
+    launch_k(paged_join_kernel<__half, TR, 1>, dim3(MMA_WORKERS, (TR + 15) / 16), dim3(256), 0, stream, p, 1);
     return 2;
 }
 
@@ -103,6 +147,10 @@ int launch_phase(paged_params_t& p, int dtype, bool vec, cudaStream_t stream)
 {
     p.packed_min = 0;
     p.packed_max = 0x7fffffff;
+    if (dtype == ES_F16 && vec && p.d <= 128) {
+        uint32_t const rows = p.prefix_len >= 0 ? p.rows * p.group : p.group; // of an item, where tokens come singly
+        return rows <= 8 ? launch_mma<1>(p, stream) : rows <= 16 ? launch_mma<2>(p, stream) : launch_mma<4>(p, stream);
+    }
     return dtype == ES_F16 ? launch_simt<__half>(p, vec, stream) : launch_simt<float>(p, vec, stream);
 }
 
@@ -115,7 +163,7 @@ void check_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
     if (!a.heads || a.heads % c.kv_heads) fail(ES_BAD_DESCRIPTOR, "paged attention: query heads must be a multiple of the key heads");
     if (a.heads > 65535) fail(ES_NOT_SUPPORTED, "paged attention: more than 65535 heads");
     if ((uint64_t)c.rows * (a.heads / c.kv_heads) > 0x7fffffffull) fail(ES_NOT_SUPPORTED, "paged attention: too many rows");
-    if (!std::isfinite(a.scale)) fail(ES_BAD_DESCRIPTOR, "paged attention: the scale must be finite");
+    if (!(a.scale >= 1e-30f && a.scale <= 1e30f)) fail(ES_BAD_DESCRIPTOR, "paged attention: the scale must lie in 1e-30 .. 1e30");
     if (!x.q || !x.k_cache || !x.v_cache || !x.out || !x.lengths || !x.tables) fail(ES_BAD_ARGUMENT, "paged attention: null pointer");
     if (!prefix && a.prefix_len) fail(ES_BAD_ARGUMENT, "paged attention: a prefix needs es_b200_launch_prefix_attention");
     if (a.prefix_len > 0x7fffffffu) fail(ES_NOT_SUPPORTED, "paged attention: prefix beyond 31 bits");

@@ -12,7 +12,7 @@
 namespace es {
 namespace {
 
-constexpr int SIMT_BK = 64;
+constexpr int SIMT_BK = 64, SIMT_OVH = 2;
 
 // 4 elements of type T as f32; vec: one load, else the first n of them one by one
 template <typename T> __device__ __forceinline__ void load4(T const* p, float (&x)[4], bool vec, int n)
@@ -36,14 +36,14 @@ template <typename T> __device__ __forceinline__ void load4(T const* p, float (&
 template <typename T, int NCH, bool VEC> // NCH: chunks of 32 elements of the head dim
 __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__ paged_params_t p)
 {
-    constexpr int TR = 16 / NCH, BK = SIMT_BK, NT = 128;
-    __shared__ sched_smem_t<NT> sched;
+    constexpr int TR = 16 / NCH, BK = SIMT_BK, OVH = SIMT_OVH, NT = 128;
+    __shared__ sched_smem_t<NT, 1> sched;
     __shared__ float            so[4][TR][NCH * 32];
     __shared__ float2           sml[4][TR];
     ES_PDL_PROLOGUE();
     int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, stream = threadIdx.x >> 3;
     work_t    w;
-    find_work<TR, BK, NT>(p, w, sched);
+    find_work<TR, BK, OVH, NT, 1>(p, w, sched);
     bool split = false;
     while (w.left) {
         uint32_t const n_units = min(w.kt - w.j, w.left);
@@ -71,7 +71,8 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
                 for (int i = 0; i < 4; ++i) q[r][c][i] *= p.scale_log2;
             }
         }
-        int const key_end = (int)min((uint64_t)(w.j + n_units) * BK, (uint64_t)vis_max);
+        int const key_begin = (int)(first_tile_of<OVH>(w.j) * BK);
+        int const key_end = (int)min((uint64_t)first_tile_of<OVH>(w.j + n_units) * BK, (uint64_t)vis_max);
         T const*  kb = static_cast<T const*>(p.k) + (int64_t)w.head * p.k_stride[2];
         T const*  vb = static_cast<T const*>(p.v) + (int64_t)w.head * p.v_stride[2];
         auto      load = [&](int key, float (&k)[NCH][4], float (&v)[NCH][4]) -> bool {
@@ -98,10 +99,10 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
             return true;
         };
         float     k[NCH][4], v[NCH][4];
-        int const key0 = (int)(w.j * BK) + stream;
+        int const key0 = key_begin + stream;
         bool      have = load(key0, k, v);
         // (every group of the warp makes the same number of rounds: the shuffles are the warp's)
-        int const rounds = key_end > (int)(w.j * BK) ? (key_end - (int)(w.j * BK) + 15) / 16 : 0;
+        int const rounds = key_end > key_begin ? (key_end - key_begin + 15) / 16 : 0;
         for (int i = 0; i < rounds; ++i) {
             int const key = key0 + i * 16;
             float     kn[NCH][4], vn[NCH][4];
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
                 s += __shfl_xor_sync(0xffffffffu, s, 1);
                 if (have && key < vis[r]) {
                     if (s > m[r]) {
-                        float const a = exp2f(m[r] - s); // m = -inf: 0
+                        float const a = ex2(m[r] - s); // m = -inf: 0
                         m[r] = s;
                         l[r] *= a;
 #pragma unroll
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
 #pragma unroll
                             for (int x = 0; x < 4; ++x) o[r][c][x] *= a;
                     }
-                    float const e = exp2f(s - (m[r] == -INFINITY ? 0.f : m[r]));
+                    float const e = ex2(s - (m[r] == -INFINITY ? 0.f : m[r]));
                     l[r] += e;
 #pragma unroll
                     for (int c = 0; c < NCH; ++c)
@@ -150,8 +151,8 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
             for (int x = 8; x <= 16; x <<= 1) {
                 float const mo = __shfl_xor_sync(0xffffffffu, m[r], x), lo = __shfl_xor_sync(0xffffffffu, l[r], x);
                 float const mn = fmaxf(m[r], mo);
-                float const a = m[r] == -INFINITY ? (l[r] == 0.f ? 0.f : 1.f) : exp2f(m[r] - mn);
-                float const b = mo == -INFINITY ? (lo == 0.f ? 0.f : 1.f) : exp2f(mo - mn);
+                float const a = m[r] == -INFINITY ? (l[r] == 0.f ? 0.f : 1.f) : ex2(m[r] - mn);
+                float const b = mo == -INFINITY ? (lo == 0.f ? 0.f : 1.f) : ex2(mo - mn);
                 l[r] = l[r] * a + lo * b;
 #pragma unroll
                 for (int c = 0; c < NCH; ++c)
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
             for (int i = 0; i < 4; ++i) {
                 float2 const ml = sml[i][r];
                 if (ml.y == 0.f) continue;
-                float const wgt = exp2f(ml.x - (top == -INFINITY ? 0.f : top));
+                float const wgt = ex2(ml.x - (top == -INFINITY ? 0.f : top));
                 float4 const a = *reinterpret_cast<float4 const*>(&so[i][r][e]);
                 ls = fmaf(ml.y, wgt, ls);
                 sum[0] = fmaf(a.x, wgt, sum[0]);
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
             split = true;
             if (threadIdx.x == 0) write_meta<TR>(p, w, true);
         }
-        next_item<TR, BK>(p, w, n_units);
+        next_item<TR, BK, OVH>(p, w, n_units);
     }
     if (!split && !p.direct && threadIdx.x == 0) write_meta<TR>(p, w, false);
 }

@@ -15,6 +15,13 @@
 namespace es {
 namespace {
 
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 constexpr float LOG2_E = 1.4426950408889634f;
 constexpr float LN_2 = 0.6931471805599453f;
 
@@ -29,17 +36,17 @@ struct paged_params_t {
     int32_t const* tables;
     float const*   base_out;    // result over a prefix [rows, heads, d], merged in; may be null
     float const*   base_lse;
-    float*         part_out;    // [blocks][2][TR][part_d]
-    float2*        part_ml;     // [blocks][2][TR]: maximum (log2 units), sum
-    int4*          meta;        // [blocks][2]
+    float*         part_out;    // [workers][2][TR][part_d]
+    float2*        part_ml;     // [workers][2][TR]: maximum (log2 units), sum
+    int4*          meta;        // [workers][2]
     int64_t        q_stride[2], out_stride[2], k_stride[3], v_stride[3];
     uint32_t       batch, rows, heads, kv_heads, group, d, part_d, n_pages, table_stride, capacity;
     fastdiv_t      page, grp;
     int32_t        causal;
     int32_t        prefix_len;  // >= 0: all rows attend the one list of pages `tables`, of this many tokens
-    int32_t        direct;      // one block an item: nothing is split (one row a sequence)
+    int32_t        direct;      // one worker an item: nothing is split (one row a sequence)
     uint32_t       packed_min, packed_max; // sequences with more than / at most so many packed rows
-    uint32_t       min_units;   // a block's share is at least this
+    uint32_t       min_units;   // a worker's share is at least this
     float          scale_log2;  // scale * log2 e
     int32_t        out_f32;
     unsigned int*  error;
@@ -102,12 +109,12 @@ __device__ __forceinline__ int visible(paged_params_t const& p, sequence_t const
     return p.causal ? max(0, min(s.len, s.len - s.n + tok + 1)) : s.len;
 }
 
-// key tiles of the sequence's row tile t: those that its last token sees, one at least (it writes the result)
-template <int TR, int BK> __device__ __forceinline__ uint32_t tile_units(paged_params_t const& p, sequence_t const& s, uint32_t t)
+// units of the sequence's row tile t: the key tiles that its last token sees, one at least, and OVH in front
+template <int TR, int BK, int OVH> __device__ __forceinline__ uint32_t tile_units(paged_params_t const& p, sequence_t const& s, uint32_t t)
 {
     uint32_t const last = min((t + 1) * TR, (uint32_t)s.n * p.group) - 1;
     uint32_t const keys = (uint32_t)visible(p, s, (int)fdivide(last, p.grp));
-    return max(1u, (keys + BK - 1) / BK);
+    return max(1u, (keys + BK - 1) / BK) + OVH;
 }
 template <int TR> __device__ __forceinline__ uint32_t row_tiles(paged_params_t const& p, sequence_t const& s)
 {
@@ -116,11 +123,11 @@ template <int TR> __device__ __forceinline__ uint32_t row_tiles(paged_params_t c
 
 // Units of one head of the lane's sequence.  Causal parts of several tokens have row tiles of different
 // length: those are summed by the whole warp, one lane's sequence after the other.  All 32 lanes call.
-template <int TR, int BK> __device__ __forceinline__ uint64_t head_units(paged_params_t const& p, sequence_t const& s)
+template <int TR, int BK, int OVH> __device__ __forceinline__ uint64_t head_units(paged_params_t const& p, sequence_t const& s)
 {
     uint64_t   u = 0;
     bool const even = s.n <= 1 || !p.causal;
-    if (s.n > 0 && even) u = (uint64_t)row_tiles<TR>(p, s) * tile_units<TR, BK>(p, s, 0);
+    if (s.n > 0 && even) u = (uint64_t)row_tiles<TR>(p, s) * tile_units<TR, BK, OVH>(p, s, 0);
     unsigned todo = __ballot_sync(0xffffffffu, s.n > 0 && !even);
     int const lane = threadIdx.x & 31;
     while (todo) {
@@ -130,7 +137,7 @@ template <int TR, int BK> __device__ __forceinline__ uint64_t head_units(paged_p
         o.len = __shfl_sync(0xffffffffu, s.len, src);
         uint32_t const rt = row_tiles<TR>(p, o);
         uint64_t       sum = 0;
-        for (uint32_t t = lane; t < rt; t += 32) sum += tile_units<TR, BK>(p, o, t);
+        for (uint32_t t = lane; t < rt; t += 32) sum += tile_units<TR, BK, OVH>(p, o, t);
 #pragma unroll
         for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
         if (lane == src) u = sum;
@@ -139,42 +146,50 @@ template <int TR, int BK> __device__ __forceinline__ uint64_t head_units(paged_p
     return u;
 }
 
-// A block's place in the work
+// A worker's place in the work
 struct work_t {
     uint32_t   seq, head, t, rt;
-    uint32_t   j, kt;   // next key tile of the item, number of its key tiles
-    uint32_t   left;    // units of this block's share still to do
+    uint32_t   j, kt;   // next unit of the item, number of its units
+    uint32_t   left;    // units of this worker's share still to do
     uint64_t   unit;    // number of the next unit
     uint32_t   chunk;   // units a share
+    uint32_t   worker;
     sequence_t s;
 };
 
-template <int NT> struct sched_smem_t {
+template <int NT, int WPB> struct sched_smem_t {
     uint64_t warp_sum[NT / 32];
-    uint64_t found_off;
-    uint32_t found_seq;
+    uint64_t found_off[WPB];
+    uint32_t found_seq[WPB];
 };
 
-// All NT threads call; blockIdx.x is the block's number among gridDim.x.
-template <int TR, int BK, int NT>
-__device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sched_smem_t<NT>& sm)
+// All NT threads call.  WPB workers a block: 1, or its NT / 32 warps.
+template <int TR, int BK, int OVH, int NT, int WPB>
+__device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sched_smem_t<NT, WPB>& sm)
 {
+    static_assert(WPB == 1 || WPB == NT / 32, "a worker is a block or a warp");
     int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int const mine_in_block = WPB == 1 ? 0 : warp;
+    w.worker = blockIdx.x * WPB + mine_in_block;
     uint32_t const n_seq = p.prefix_len >= 0 ? 1u : p.batch;
     w.left = 0;
     w.j = 0;
     w.unit = 0;
     w.chunk = 0xffffffffu;
     if (p.direct) {
-        // one row a sequence: item number = (sequence, head, row tile), nothing to count
+        // one row a sequence: blocks (items of a sequence, sequences); nothing to count
         w.rt = (p.group + TR - 1) / TR;
-        uint32_t const b = blockIdx.x;
-        w.t = b % w.rt;
-        w.head = (b / w.rt) % p.kv_heads;
-        w.seq = b / w.rt / p.kv_heads;
+        w.head = w.worker;
+        w.t = 0;
+        if (w.rt > 1) {
+            w.head = w.worker / w.rt;
+            w.t = w.worker - w.head * w.rt;
+        }
+        w.seq = blockIdx.y;
+        if (w.head >= p.kv_heads) return;
         w.s = get_sequence(p, w.seq);
         if (w.s.n == 0) return;
-        w.kt = tile_units<TR, BK>(p, w.s, w.t);
+        w.kt = tile_units<TR, BK, OVH>(p, w.s, w.t);
         w.left = w.kt;
         return;
     }
@@ -184,7 +199,7 @@ __device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sc
         s.n = 0;
         s.len = 0;
         if (i0 + threadIdx.x < n_seq) s = get_sequence(p, i0 + threadIdx.x);
-        u0 = head_units<TR, BK>(p, s) * p.kv_heads;
+        u0 = head_units<TR, BK, OVH>(p, s) * p.kv_heads;
         mine += u0;
     }
 #pragma unroll
@@ -195,13 +210,13 @@ __device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sc
 #pragma unroll
     for (int i = 0; i < NT / 32; ++i) total += sm.warp_sum[i];
     __syncthreads();
-    uint64_t const share = max((total + gridDim.x - 1) / gridDim.x, (uint64_t)p.min_units);
+    uint64_t const share = max((total + gridDim.x * WPB - 1) / (gridDim.x * WPB), (uint64_t)p.min_units);
     w.chunk = (uint32_t)min(share, (uint64_t)0xffffffffu);
-    uint64_t const lo = (uint64_t)blockIdx.x * w.chunk;
-    if (lo >= total) return; // (uniform)
-    w.unit = lo;
-    w.left = (uint32_t)min((uint64_t)w.chunk, total - lo);
-    // the sequence that holds unit `lo`
+    uint64_t const lo0 = (uint64_t)blockIdx.x * WPB * w.chunk; // the block's first worker's first unit
+    if (lo0 >= total) return;                                  // (the block has no work)
+    uint64_t const lo = lo0 + (uint64_t)mine_in_block * w.chunk;
+    uint64_t const lo_last = min(lo0 + (uint64_t)(WPB - 1) * w.chunk, total - 1);
+    // the sequences that hold the workers' first units
     uint64_t base = 0;
     for (uint32_t i0 = 0; i0 < n_seq; i0 += NT) {
         uint64_t u = u0;
@@ -210,7 +225,7 @@ __device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sc
             s.n = 0;
             s.len = 0;
             if (i0 + threadIdx.x < n_seq) s = get_sequence(p, i0 + threadIdx.x);
-            u = head_units<TR, BK>(p, s) * p.kv_heads;
+            u = head_units<TR, BK, OVH>(p, s) * p.kv_heads;
         }
         uint64_t incl = u;
 #pragma unroll
@@ -227,30 +242,37 @@ __device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sc
             all += sm.warp_sum[i];
         }
         incl += before;
-        if (lo < incl && lo >= incl - u) {
-            sm.found_seq = i0 + threadIdx.x;
-            sm.found_off = lo - (incl - u);
+#pragma unroll
+        for (int x = 0; x < WPB; ++x) {
+            uint64_t const first = lo0 + (uint64_t)x * w.chunk;
+            if (first < incl && first >= incl - u) {
+                sm.found_seq[x] = i0 + threadIdx.x;
+                sm.found_off[x] = first - (incl - u);
+            }
         }
         base += all;
         __syncthreads();
-        if (lo < base) break; // (uniform)
+        if (lo_last < base) break; // (the same in the whole block)
     }
-    w.seq = sm.found_seq;
-    uint64_t off = sm.found_off;
+    if (lo >= total) return; // this warp has no work
+    w.unit = lo;
+    w.left = (uint32_t)min((uint64_t)w.chunk, total - lo);
+    w.seq = sm.found_seq[mine_in_block];
+    uint64_t off = sm.found_off[mine_in_block];
     w.s = get_sequence(p, w.seq);
-    uint64_t const per_head = head_units<TR, BK>(p, w.s); // every lane of every warp has the same sequence
+    uint64_t const per_head = head_units<TR, BK, OVH>(p, w.s); // every lane of every warp has the same sequence
     w.head = (uint32_t)(off / per_head);
     off -= w.head * per_head;
     w.rt = row_tiles<TR>(p, w.s);
     if (w.s.n <= 1 || !p.causal) {
-        w.kt = tile_units<TR, BK>(p, w.s, 0);
+        w.kt = tile_units<TR, BK, OVH>(p, w.s, 0);
         w.t = (uint32_t)(off / w.kt);
         w.j = (uint32_t)(off - (uint64_t)w.t * w.kt);
         return;
     }
     for (uint32_t t0 = 0;; t0 += 32) {
         uint32_t const t = t0 + lane;
-        uint64_t const u = t < w.rt ? tile_units<TR, BK>(p, w.s, t) : 0;
+        uint64_t const u = t < w.rt ? tile_units<TR, BK, OVH>(p, w.s, t) : 0;
         uint64_t       incl = u;
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
@@ -270,7 +292,7 @@ __device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sc
 }
 
 // The next item, after `done` units of this one
-template <int TR, int BK> __device__ __forceinline__ void next_item(paged_params_t const& p, work_t& w, uint32_t done)
+template <int TR, int BK, int OVH> __device__ __forceinline__ void next_item(paged_params_t const& p, work_t& w, uint32_t done)
 {
     w.left -= done;
     w.unit += done;
@@ -286,21 +308,37 @@ template <int TR, int BK> __device__ __forceinline__ void next_item(paged_params
             w.rt = row_tiles<TR>(p, w.s);
         }
     }
-    w.kt = tile_units<TR, BK>(p, w.s, w.t);
+    w.kt = tile_units<TR, BK, OVH>(p, w.s, w.t);
 }
 
-// Where a segment's result goes: -1 finished here, 0 / 1 the block's first / last partial result
+// Key tiles [first, end) among the item's units [j, j + n)
+template <int OVH> __device__ __forceinline__ uint32_t first_tile_of(uint32_t j)
+{
+    return j > OVH ? j - OVH : 0u;
+}
+// Moves over units that stand for no tile; false: the share ends among them
+template <int OVH> __device__ __forceinline__ bool to_next_tile(work_t& w)
+{
+    if (w.j < OVH) {
+        uint32_t const n = min(OVH - w.j, w.left);
+        w.j += n;
+        w.left -= n;
+    }
+    return w.left != 0;
+}
+
+// Where a segment's result goes: -1 finished here, 0 / 1 the worker's first / last partial result
 __device__ __forceinline__ int segment_slot(work_t const& w, uint32_t n)
 {
     if (w.j == 0 && n == w.kt) return -1;
     return w.j == 0 ? 1 : 0;
 }
 
-// Every block says whether its last item goes on in the following blocks (thread 0)
+// Every worker says whether its last item goes on in the following shares (one thread)
 template <int TR>
 __device__ __forceinline__ void write_meta(paged_params_t const& p, work_t const& w, bool split)
 {
-    int4* m = p.meta + 2 * blockIdx.x;
+    int4* m = p.meta + 2 * (uint64_t)w.worker;
     if (!split) {
         m[0] = make_int4(0, 0, 0, 0);
         return;
@@ -328,12 +366,13 @@ __device__ __forceinline__ finish_t finish(float m, float l, bool has_base, floa
         f.lse = -INFINITY;
         return f;
     }
-    float const a = l == 0.f ? 0.f : exp2f(m - top);
-    float const b = b2 == -INFINITY ? 0.f : exp2f(b2 - top);
-    float const total = fmaf(l, a, b);
-    f.wa = a / total;
-    f.wb = b / total;
-    f.lse = (top + log2f(total)) * LN_2;
+    // (the hardware's 2^x, log2 and reciprocal: a few steps of 2^-23)
+    float const a = l == 0.f ? 0.f : ex2(m - top);
+    float const b = b2 == -INFINITY ? 0.f : ex2(b2 - top);
+    float const total = fmaf(l, a, b), inv = __fdividef(1.f, total);
+    f.wa = a * inv;
+    f.wb = b * inv;
+    f.lse = (top + __log2f(total)) * LN_2;
     return f;
 }
 
@@ -382,58 +421,116 @@ __device__ __forceinline__ void write_out(paged_params_t const& p, int row, uint
 }
 
 // Joins the partial results of the items that crossed shares.  Block x: the item that starts last in share x
-// (if it goes on behind it); a warp a row; lanes over the head dim.
-template <typename T, int TR>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ paged_params_t p, int aligned)
+// (if it goes on behind it); block y: 16 rows of it.  A warp takes a row, or with fewer rows than warps every
+// SLICES-th part of one; lanes over the head dim.  The parts' weights are found 32 at a time, a lane a part, so
+// that the loads of the parts' sums wait for nothing but each other.
+template <typename T, int TR, int CHUNKS> // CHUNKS: of 128 elements of the head dim
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ paged_params_t p, int aligned)
 {
+    constexpr uint32_t WARPS = 8;
+    constexpr int      BATCH = 8 / CHUNKS;
+    __shared__ float   so[WARPS][CHUNKS * 128];
+    __shared__ float2  sml[WARPS];
     ES_PDL_PROLOGUE();
     int4 const     m0 = p.meta[2 * blockIdx.x];
-    uint32_t const r = blockIdx.y * 4 + (threadIdx.x >> 5);
-    if (r >= (uint32_t)m0.x) return;
-    int const      last = p.meta[2 * blockIdx.x + 1].x;
-    uint32_t const lane = threadIdx.x & 31;
-    int const      first = (int)blockIdx.x, n = last - first + 1;
-    // part i lies in share first + i: its last slot for i = 0, the first slot of the others
-    auto slot = [&](int i) { return (uint64_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * TR + r; };
-    float top = -INFINITY;
-    for (int i = (int)lane; i < n; i += 32) {
-        float2 const ml = p.part_ml[slot(i)];
-        if (ml.y != 0.f) top = fmaxf(top, ml.x);
-    }
+    uint32_t const r0 = blockIdx.y * 16;
+    if (r0 >= (uint32_t)m0.x) return;
+    int const      first = (int)blockIdx.x, n = p.meta[2 * blockIdx.x + 1].x - first + 1;
+    uint32_t const rows = min((uint32_t)m0.x - r0, 16u), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t const at_once = min(rows, WARPS), slices = WARPS / at_once, slice = warp / at_once;
+    for (uint32_t rr = 0; rr < rows; rr += at_once) {
+        uint32_t const r = r0 + rr + warp % at_once;
+        bool const     on = slice < slices && r < r0 + rows;
+        // part i lies in share first + i: its last slot for i = 0, the first slot of the others
+        auto  slot = [&](int i) { return (uint64_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * TR + r; };
+        float top = -INFINITY, l = 0.f, o[CHUNKS][4] = {};
+        if (on) {
+            for (int i0 = (int)slice * 32; i0 < n; i0 += (int)slices * 32) {
+                int const    i = i0 + (int)lane;
+                float2 const ml = i < n ? p.part_ml[slot(i)] : make_float2(-INFINITY, 0.f);
+                float        tm = ml.y == 0.f ? -INFINITY : ml.x;
 #pragma unroll
-    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    float o[2][4] = {}, l = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        float2 const ml = p.part_ml[slot(i)];
-        if (ml.y == 0.f) continue; // no key
-        float const  wgt = exp2f(ml.x - top);
-        float const* src = p.part_out + slot(i) * p.part_d;
-        l = fmaf(ml.y, wgt, l);
+                for (int x = 16; x; x >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, x));
+                if (tm > top) {
+                    float const a = ex2(top - tm); // top = -inf: 0
+                    l *= a;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            uint32_t const e = c * 128 + lane * 4;
-            if (e < p.part_d) {
-                float4 const x = *reinterpret_cast<float4 const*>(src + e);
-                o[c][0] = fmaf(x.x, wgt, o[c][0]);
-                o[c][1] = fmaf(x.y, wgt, o[c][1]);
-                o[c][2] = fmaf(x.z, wgt, o[c][2]);
-                o[c][3] = fmaf(x.w, wgt, o[c][3]);
+                    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[c][k] *= a;
+                    top = tm;
+                }
+                float const wgt = ml.y == 0.f ? 0.f : ex2(ml.x - (top == -INFINITY ? 0.f : top));
+                float       ls = ml.y * wgt;
+#pragma unroll
+                for (int x = 16; x; x >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
+                l += ls;
+                int const here = min(32, n - i0);
+                for (int k0 = 0; k0 < here; k0 += BATCH) { // (parts beyond the last: weight 0)
+                    float4 x[BATCH][CHUNKS];
+                    float  wk[BATCH];
+#pragma unroll
+                    for (int k = 0; k < BATCH; ++k) {
+                        float const* src = p.part_out + slot(i0 + min(k0 + k, here - 1)) * p.part_d;
+                        wk[k] = __shfl_sync(0xffffffffu, wgt, k0 + k);
+#pragma unroll
+                        for (int c = 0; c < CHUNKS; ++c)
+                            if (c * 128 + lane * 4 < p.part_d) x[k][c] = *reinterpret_cast<float4 const*>(src + c * 128 + lane * 4);
+                    }
+#pragma unroll
+                    for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+                        for (int c = 0; c < CHUNKS; ++c)
+                            if (k0 + k < here) {
+                                o[c][0] = fmaf(x[k][c].x, wk[k], o[c][0]);
+                                o[c][1] = fmaf(x[k][c].y, wk[k], o[c][1]);
+                                o[c][2] = fmaf(x[k][c].z, wk[k], o[c][2]);
+                                o[c][3] = fmaf(x[k][c].w, wk[k], o[c][3]);
+                            }
+                }
             }
         }
-    }
-    uint32_t const pr = (uint32_t)m0.z + r;
-    uint32_t const tok = fdivide(pr, p.grp);
-    int const      row = m0.y + (int)tok;
-    uint32_t const head = (uint32_t)m0.w * p.group + (pr - tok * p.group);
-    uint64_t const at = (uint64_t)row * p.heads + head;
-    finish_t const f = finish(top, l, p.base_lse != nullptr, p.base_lse ? p.base_lse[at] : 0.f);
+        if (slices > 1) { // (the same in the whole block; then all rows are done in this one round)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        uint32_t const e = c * 128 + lane * 4;
-        if (e < p.d) write_out<T, 4>(p, row, head, e, o[c], f, aligned != 0);
+            for (int c = 0; c < CHUNKS; ++c) *reinterpret_cast<float4*>(&so[warp][c * 128 + lane * 4]) = make_float4(o[c][0], o[c][1], o[c][2], o[c][3]);
+            if (lane == 0) sml[warp] = make_float2(top, l);
+            __syncthreads();
+            if (warp >= at_once) return;
+            float all = -INFINITY;
+            for (uint32_t x = 0; x < slices; ++x)
+                if (sml[warp + x * at_once].y != 0.f) all = fmaxf(all, sml[warp + x * at_once].x);
+            float sum[CHUNKS][4] = {};
+            l = 0.f;
+            for (uint32_t x = 0; x < slices; ++x) {
+                float2 const ml = sml[warp + x * at_once];
+                if (ml.y == 0.f) continue;
+                float const wgt = ex2(ml.x - (all == -INFINITY ? 0.f : all));
+                l = fmaf(ml.y, wgt, l);
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) sum[c][k] = fmaf(so[warp + x * at_once][c * 128 + lane * 4 + k], wgt, sum[c][k]);
+            }
+            top = all;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[c][k] = sum[c][k];
+        }
+        if (!on) continue;
+        uint32_t const pr = (uint32_t)m0.z + r;
+        uint32_t const tok = fdivide(pr, p.grp);
+        int const      row = m0.y + (int)tok;
+        uint32_t const head = (uint32_t)m0.w * p.group + (pr - tok * p.group);
+        uint64_t const at = (uint64_t)row * p.heads + head;
+        finish_t const f = finish(top, l, p.base_lse != nullptr, p.base_lse ? p.base_lse[at] : 0.f);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            uint32_t const e = c * 128 + lane * 4;
+            if (e < p.d) write_out<T, 4>(p, row, head, e, o[c], f, aligned != 0);
+        }
+        if (p.lse && lane == 0) p.lse[at] = f.lse;
     }
-    if (p.lse && lane == 0) p.lse[at] = f.lse;
 }
 
 } // namespace

@@ -18,17 +18,23 @@ from .einsummable import CASTABLE_CODE, einsummable_t, fill_t, touch_t
 from .scalarop import DTYPE_CODE
 
 
-_byref = ctypes.byref
+# es_cache_append_args_t / es_paged_attention_args_t: addresses one after the other (packing them takes a fifth
+# of the time of filling a ctypes structure, which counts beside kernels of a few microseconds)
+_pack9 = struct.Struct("9P").pack
+_pack10 = struct.Struct("10P").pack
 
 
 def _ptr(x):
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
+    try:
         return x.data_ptr()
-    raise TypeError("expected a device pointer (int) or a torch tensor")
+    except AttributeError:
+        raise TypeError("expected a device pointer (int) or a torch tensor") from None
+
+
+def _adr(x):
+    return 0 if x is None else _ptr(x)
 
 
 def _stream(s):
@@ -36,9 +42,10 @@ def _stream(s):
         return None
     if isinstance(s, int):
         return s or None
-    if hasattr(s, "cuda_stream"):
+    try:
         return s.cuda_stream or None
-    raise TypeError("expected a cudaStream_t (int), a torch stream or None")
+    except AttributeError:
+        raise TypeError("expected a cudaStream_t (int), a torch stream or None") from None
 
 
 def scalar_bytes(value, dtype):
@@ -208,9 +215,9 @@ class kernel_manager_t:
         rotated into q_out.  `desc` is a cache_append_t (einsummable_b200.paged); lengths [batch] count the new
         tokens already, tables [batch, table_stride] and row_offsets [batch + 1] (None: one row a sequence) are
         int32 on the device, freqs the complex64 table [n_positions, rotary_dim / 2]."""
-        x = _lib.es_cache_append_args_t(_ptr(q), _ptr(k), _ptr(v), _ptr(freqs), _ptr(q_out), _ptr(k_cache), _ptr(v_cache),
-                                        _ptr(row_offsets), _ptr(lengths), _ptr(tables))
-        _lib.check(self._lib.es_b200_launch_cache_append(self._h, _byref(desc.c), _byref(x), _stream(stream)))
+        x = _pack10(_adr(q), _ptr(k), _ptr(v), _adr(freqs), _adr(q_out), _ptr(k_cache), _ptr(v_cache), _adr(row_offsets),
+                    _ptr(lengths), _ptr(tables))
+        _lib.check(self._lib.es_b200_launch_cache_append(self._h, desc.ref, x, _stream(stream)))
 
     def paged_attention_workspace(self, desc):
         """Bytes of workspace that an attention over the paged cache needs (a paged_attention_t)."""
@@ -223,19 +230,18 @@ class kernel_manager_t:
         """Attention of the step's queries to their own sequences' keys in the cache; lse [rows, heads] f32 gets
         the logarithm of the sums of exponentials.  `desc` is a paged_attention_t (einsummable_b200.paged), the
         arrays as for cache_append, workspace = (device memory, bytes)."""
-        x = _lib.es_paged_attention_args_t(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(lse), _ptr(row_offsets),
-                                           _ptr(lengths), _ptr(tables), None)
+        x = _pack9(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _adr(lse), _adr(row_offsets), _ptr(lengths), _ptr(tables), 0)
         ws, n = (None, 0) if workspace is None else (_ptr(workspace[0]), int(workspace[1]))
-        _lib.check(self._lib.es_b200_launch_paged_attention(self._h, _byref(desc.c), _byref(x), ws, n, _stream(stream)))
+        _lib.check(self._lib.es_b200_launch_paged_attention(self._h, desc.ref, x, ws, n, _stream(stream)))
 
     def prefix_attention(self, desc, stream, out, q, k_cache, v_cache, prefix_pages, lengths, tables, row_offsets=None,
                          lse=None, workspace=None):
         """The same behind a prefix that all sequences share: its desc.prefix_len tokens lie in the pages
         prefix_pages (int32 on the device) and are read once for the whole batch."""
-        x = _lib.es_paged_attention_args_t(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(lse), _ptr(row_offsets),
-                                           _ptr(lengths), _ptr(tables), _ptr(prefix_pages))
+        x = _pack9(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _adr(lse), _adr(row_offsets), _ptr(lengths), _ptr(tables),
+                   _adr(prefix_pages))
         ws, n = (None, 0) if workspace is None else (_ptr(workspace[0]), int(workspace[1]))
-        _lib.check(self._lib.es_b200_launch_prefix_attention(self._h, _byref(desc.c), _byref(x), ws, n, _stream(stream)))
+        _lib.check(self._lib.es_b200_launch_prefix_attention(self._h, desc.ref, x, ws, n, _stream(stream)))
 
     def rowsum_f32_noalloc(self, stream, out, inn, rows, cols):
         """out[a] = sum_b inn[a,b] for f32 without any device allocation: the

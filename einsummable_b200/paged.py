@@ -6,6 +6,8 @@ llama/modules.cc:285-383); here a layer's cache is a set of pages, a sequence a 
 kernel_manager_t.cache_append / paged_attention / prefix_attention and the program_t.add_* ops of the same
 names take these descriptors with the arrays of a step.  A descriptor is built once and used every step.
 """
+import ctypes
+
 from . import _lib
 from .scalarop import DTYPE_CODE
 
@@ -52,6 +54,7 @@ class cache_append_t:
         _strides(c.v_stride, v_stride, "v_stride")
         _strides(c.q_out_stride, q_out_stride, "q_out_stride")
         self.c = c
+        self.ref = ctypes.byref(c)
 
 
 class paged_attention_t:
@@ -65,3 +68,4 @@ class paged_attention_t:
         _strides(c.q_stride, q_stride, "q_stride")
         _strides(c.out_stride, out_stride, "out_stride")
         self.c = c
+        self.ref = ctypes.byref(c)
