@@ -13,6 +13,7 @@
 #include "paged.h"
 #include "paged_mma.h"
 #include "paged_simt.h"
+#include "paged_wide.h"
 #include "paged_work.h"
 
 namespace es {
@@ -23,6 +24,7 @@ __device__ unsigned int g_paged_error;
 
 constexpr uint32_t SIMT_BLOCKS = 2 * SM_COUNT;
 constexpr uint32_t MMA_BLOCKS = 2 * SM_COUNT, MMA_WORKERS = MMA_BLOCKS * MMA_WARPS, MMA_MAX_TR = 32;
+constexpr uint32_t WIDE_BLOCKS = SM_COUNT;
 
 uint64_t align256(uint64_t x)
 {
@@ -43,6 +45,8 @@ layout_t layout(es_paged_attention_t const& a)
         part = std::max<uint64_t>(part, 2ull * MMA_WORKERS * MMA_MAX_TR * (c.head_dim <= 64 ? 64 : 128));
         ml = std::max<uint64_t>(ml, 2ull * MMA_WORKERS * MMA_MAX_TR);
         meta = std::max<uint64_t>(meta, MMA_WORKERS);
+        part = std::max<uint64_t>(part, 2ull * WIDE_BLOCKS * WIDE_TR * (c.head_dim <= 64 ? 64 : 128));
+        ml = std::max<uint64_t>(ml, 2ull * WIDE_BLOCKS * WIDE_TR);
     }
     uint64_t at = 0;
     l.part_out = at;
@@ -143,15 +147,50 @@ template <int NT> int launch_mma(paged_params_t& p, cudaStream_t stream)
     return 2;
 }
 
+template <int DPAD> void launch_wide_as(paged_params_t const& p, cudaStream_t stream)
+{
+    static bool done[64] = {};
+    allow_smem(paged_wide_kernel<DPAD>, wide_smem_bytes<DPAD>(), done);
+    launch_k(paged_wide_kernel<DPAD>, dim3(WIDE_BLOCKS), dim3(WIDE_THREADS), wide_smem_bytes<DPAD>(), stream, p);
+}
+
+int launch_wide(paged_params_t& p, cudaStream_t stream)
+{
+    p.part_d = p.d <= 64 ? 64 : 128;
+    p.direct = 0;
+    p.min_units = 4;
+    if (p.part_d == 64) launch_wide_as<64>(p, stream);
+    else launch_wide_as<128>(p, stream);
+    pdl_scope_t scope(true);
+    launch_k(paged_join_kernel<__half, WIDE_TR, 1>, dim3(WIDE_BLOCKS, WIDE_TR / 16), dim3(256), 0, stream, p, 1);
+    return 2;
+}
+
+// f16 on the tensor cores: sequences (or the prefix) with up to MMA_MAX_TR packed rows a key head are bound by
+// memory and go to the warp-level units, those with more to tcgen05.  How many rows a sequence has is known on
+// the device when there are row offsets: then both kernels run and each takes its own.
 int launch_phase(paged_params_t& p, int dtype, bool vec, cudaStream_t stream)
 {
     p.packed_min = 0;
     p.packed_max = 0x7fffffff;
-    if (dtype == ES_F16 && vec && p.d <= 128) {
-        uint32_t const rows = p.prefix_len >= 0 ? p.rows * p.group : p.group; // of an item, where tokens come singly
-        return rows <= 8 ? launch_mma<1>(p, stream) : rows <= 16 ? launch_mma<2>(p, stream) : launch_mma<4>(p, stream);
+    if (dtype != ES_F16) return launch_simt<float>(p, vec, stream);
+    if (!vec || p.d > 128) return launch_simt<__half>(p, vec, stream);
+    bool const     counted = p.prefix_len < 0 && !p.row_offsets;  // one row a sequence
+    uint32_t const most = counted ? p.group : p.rows * p.group;   // packed rows of an item
+    uint32_t const fewest = counted ? p.group : 1;
+    int            launches = 0;
+    if (fewest <= MMA_MAX_TR) {
+        p.packed_max = MMA_MAX_TR;
+        uint32_t const rows = p.prefix_len >= 0 ? most : p.group; // of an item, where tokens come singly
+        launches += rows <= 8 ? launch_mma<1>(p, stream) : rows <= 16 ? launch_mma<2>(p, stream) : launch_mma<4>(p, stream);
     }
-    return dtype == ES_F16 ? launch_simt<__half>(p, vec, stream) : launch_simt<float>(p, vec, stream);
+    if (most > MMA_MAX_TR) {
+        pdl_scope_t scope(launches > 0 || pdl_launch_flag());
+        p.packed_min = MMA_MAX_TR;
+        p.packed_max = 0x7fffffff;
+        launches += launch_wide(p, stream);
+    }
+    return launches;
 }
 
 } // namespace

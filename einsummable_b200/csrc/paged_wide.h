@@ -1,0 +1,439 @@
+// Paged attention for many packed rows a key head (a batch behind a shared prefix, parts of prompts), f16, on
+// the fifth-generation tensor cores.
+//
+// Bound: the tensor cores, and as much the exponentials: a tile of 128 rows x 128 keys of 128 elements is 2 * 512
+// cycles of products and, at 16 exponentials a cycle, 1024 of softmax.  So an item is two tiles of 128 packed rows
+// that share the keys in shared memory and take turns: while one tile's scores are on the tensor cores, the
+// other's are exponentials.  One persistent block an SM, 12 warps:
+//   warps 0-3, 4-7   softmax of tile 0 / 1, a thread a row (= TMEM lane): maximum of the 128 scores, rescaling of
+//                    the accumulator when it has moved by more than 2^8, exponentials (f32; rounded to f16 for
+//                    the product with the values), written as f16 pairs over the scores they came from
+//   warp 8           issues the products: S_t = Q_t K^T into TMEM, O_t += P_t V with P_t read from TMEM
+//   warps 9-11       copy the pages: 44 keys a warp, a lane finds a key's page, 16-byte asynchronous copies into
+//                    the 128-byte-swizzled tiles the tensor cores read (any page size: a tile's rows are
+//                    gathered one by one); two stages each for keys and values
+// TMEM: scores 2 x 128 columns, accumulators 2 x 128.  Products of one thread are done in order, so S_t of the
+// next tile may be issued over P_t as soon as P_t V is, and whoever sees S_t complete knows P_t V to be.
+// Every wait is bounded; on expiry the kernel records 0x31-0x38, lets its copies land, frees TMEM and returns.
+#pragma once
+#include "paged_mma.h"
+
+namespace es {
+namespace {
+
+constexpr int      WIDE_TR = 256, WIDE_BK = 128, WIDE_OVH = 2, WIDE_COPY_WARPS = 3, WIDE_THREADS = (9 + WIDE_COPY_WARPS) * 32;
+constexpr uint64_t WIDE_WAIT_LIMIT_CYCLES = 4000000000ull; // ~2 s at 2 GHz
+
+struct wide_ctrl_t {
+    uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], o_free[2];
+    uint32_t tmem_base;
+    uint32_t abort_flag;
+};
+
+__device__ __forceinline__ bool wide_wait(paged_params_t const& p, uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t code)
+{
+    if (mbar_try_wait(bar, parity)) return true;
+    long long t0 = clock64();
+    uint32_t  spins = 0;
+    while (!mbar_try_wait(bar, parity)) {
+        if ((++spins & 0x3ff) == 0) {
+            if (*abort_flag) return false;
+            if ((uint64_t)(clock64() - t0) > WIDE_WAIT_LIMIT_CYCLES) {
+                *abort_flag = code;
+                report(p, code);
+                return false;
+            }
+        }
+    }
+    return true;
+}
+
+// D (TMEM) += A (TMEM, f16 pairs) x B (shared memory)
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, uint32_t const (&r)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+template <int DPAD> constexpr uint32_t wide_smem_bytes()
+{
+    return (2 + 2 + 2) * (DPAD / 64) * 16384 + (uint32_t)sizeof(wide_ctrl_t) + 1024;
+}
+
+template <int DPAD>
+__global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __grid_constant__ paged_params_t p)
+{
+    constexpr int      TR = WIDE_TR, BK = WIDE_BK, OVH = WIDE_OVH;
+    constexpr uint32_t KB = DPAD / 64, BLOCK = 16384, TILE = KB * BLOCK; // 64-element blocks: 128 rows of 128 bytes
+    __shared__ sched_smem_t<WIDE_THREADS, 1> sched;
+    extern __shared__ uint8_t                smem_wide[];
+    uint8_t* const     smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_wide) + 1023) & ~uintptr_t(1023));
+    wide_ctrl_t* const ctrl = reinterpret_cast<wide_ctrl_t*>(smem + 6 * TILE);
+    volatile uint32_t* abort_flag = &ctrl->abort_flag;
+    uint32_t const     sQ = smem_u32(smem), sK = sQ + 2 * TILE, sV = sK + 2 * TILE; // two tiles each
+    uint32_t const     bars = smem_u32(ctrl);
+    uint32_t const     q_full = bars, q_empty = bars + 8; // in the order of wide_ctrl_t
+    uint32_t const     k_full = q_empty + 8, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16, s_full = v_empty + 16,
+                   p_ready = s_full + 16, o_done = p_ready + 16, o_free = o_done + 16;
+    int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, WIDE_COPY_WARPS * 32);
+        mbar_init(q_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(k_full + 8 * i, WIDE_COPY_WARPS * 32);
+            mbar_init(k_empty + 8 * i, 1);
+            mbar_init(v_full + 8 * i, WIDE_COPY_WARPS * 32);
+            mbar_init(v_empty + 8 * i, 1);
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_ready + 8 * i, 128);
+            mbar_init(o_done + 8 * i, 1);
+            mbar_init(o_free + 8 * i, 128);
+        }
+        ctrl->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctrl->tmem_base)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (p.d != DPAD) // columns that no copy fills: zeros
+        for (uint32_t i = threadIdx.x * 16; i < 6 * TILE; i += WIDE_THREADS * 16)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sQ + i), "r"(0) : "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t const tmem = ctrl->tmem_base; // scores: + 128 t; accumulators: + 256 + 128 t
+    ES_PDL_PROLOGUE();
+    work_t w;
+    find_work<TR, BK, OVH, WIDE_THREADS, 1>(p, w, sched);
+
+    if (warp >= 9) {
+        // ------------------------------------------------------------ copies
+        constexpr int  CH = DPAD / 8, ROWS_AT = 32 / CH;
+        int const      lw = warp - 9, c_row = lane / CH, c_chunk = lane % CH;
+        bool const     c_on = (uint32_t)c_chunk * 8 < p.d;
+        uint32_t const c_col = (uint32_t)(c_chunk >> 3) * BLOCK, cc = c_chunk & 7;
+        // groups of copies in flight, oldest first: the barrier that each completes
+        uint32_t pend[3];
+        int      n_pend = 0;
+        auto     signal = [&](uint32_t b) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(b);
+        };
+        auto flush = [&]() {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            for (int i = 0; i < n_pend; ++i) signal(pend[i]);
+            n_pend = 0;
+        };
+        auto commit = [&](uint32_t b) {
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (n_pend == 2) {
+                asm volatile("cp.async.wait_group 2;" ::: "memory");
+                signal(pend[0]);
+                pend[0] = pend[1];
+                n_pend = 1;
+            }
+            pend[n_pend++] = b;
+        };
+        auto acquire = [&](uint32_t b, uint32_t parity) { // a tile that the products no longer read
+            if (__all_sync(0xffffffffu, mbar_try_wait(b, parity))) return true;
+            flush(); // what has been copied may be what they wait for
+            return __all_sync(0xffffffffu, wide_wait(p, b, parity, abort_flag, 0x37)) != 0;
+        };
+        uint32_t items = 0, tiles = 0;
+        bool     ok = true;
+        while (w.left && ok) {
+            uint32_t const n = min(w.kt - w.j, w.left), f0 = first_tile_of<OVH>(w.j), f1 = first_tile_of<OVH>(w.j + n);
+            if (f1 > f0) {
+                uint32_t const start = w.t * TR, count = min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
+                ok = acquire(q_empty, (items & 1) ^ 1);
+                if (!ok) break;
+                for (uint32_t r = lw * ROWS_AT + c_row; r < (count + 127) / 128 * 128; r += WIDE_COPY_WARPS * ROWS_AT) {
+                    uint32_t const pr = min(start + r, start + count - 1), tok = fdivide(pr, p.grp);
+                    __half const*  src = static_cast<__half const*>(p.q) + (int64_t)(w.s.row0 + (int)tok) * p.q_stride[0] +
+                                        (int64_t)(w.head * p.group + (pr - tok * p.group)) * p.q_stride[1] + c_chunk * 8;
+                    uint32_t const dst = sQ + (r >> 7) * TILE + c_col + (r & 127) * 128 + ((cc ^ (r & 7)) << 4);
+                    if (c_on) copy16(dst, src, r < count);
+                }
+                commit(q_full);
+                ++items;
+                for (uint32_t j = f0; j < f1 && ok; ++j, ++tiles) {
+                    // where this warp's keys lie: lane x has keys x and 32 + x of its range
+                    uint32_t const range = lw * 44, range_n = min(44u, 128u - range);
+                    int64_t        ko[2] = {0, 0}, vo[2] = {0, 0};
+                    unsigned       ons[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        uint32_t const at = lane + 32 * x, key = j * BK + range + at;
+                        bool           on = at < range_n && key < (uint32_t)w.s.len;
+                        if (on) {
+                            uint32_t const pi = fdivide(key, p.page), slot = key - pi * p.page.d;
+                            uint32_t const page = (uint32_t)w.s.table[pi];
+                            on = page < p.n_pages;
+                            if (!on) report(p, PAGED_BAD_PAGE);
+                            ko[x] = (int64_t)page * p.k_stride[0] + (int64_t)slot * p.k_stride[1] + (int64_t)w.head * p.k_stride[2];
+                            vo[x] = (int64_t)page * p.v_stride[0] + (int64_t)slot * p.v_stride[1] + (int64_t)w.head * p.v_stride[2];
+                        }
+                        ons[x] = __ballot_sync(0xffffffffu, on);
+                    }
+                    uint32_t const st = tiles & 1, par = ((tiles >> 1) & 1) ^ 1;
+                    auto copy_tile = [&](uint32_t dst, void const* base, int64_t const (&off)[2]) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll 4
+                            for (int i = 0; i < 32 / ROWS_AT; ++i) {
+                                uint32_t const r = c_row + i * ROWS_AT, row = range + 32 * x + r;
+                                if (32 * x + i * ROWS_AT >= range_n) break; // (ranges are multiples of 4 rows)
+                                int64_t const at = __shfl_sync(0xffffffffu, off[x], r);
+                                bool const    live = (ons[x] >> r) & 1;
+                                if (c_on)
+                                    copy16(dst + c_col + row * 128 + ((cc ^ (row & 7)) << 4),
+                                           live ? (void const*)(static_cast<__half const*>(base) + at + c_chunk * 8) : base, live);
+                            }
+                    };
+                    if (!(ok = acquire(k_empty + 8 * st, par))) break;
+                    copy_tile(sK + st * TILE, p.k, ko);
+                    commit(k_full + 8 * st);
+                    if (!(ok = acquire(v_empty + 8 * st, par))) break;
+                    copy_tile(sV + st * TILE, p.v, vo);
+                    commit(v_full + 8 * st);
+                }
+            }
+            next_item<TR, BK, OVH>(p, w, n);
+        }
+        flush();
+    } else if (warp == 8) {
+        // ------------------------------------------------------------ products (the whole warp; one lane issues)
+        bool leader;
+        {
+            uint32_t pred;
+            asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(pred));
+            leader = pred != 0;
+        }
+        uint64_t const desc_hi = (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32; // 128B swizzle, 1024 bytes between 8-row groups
+        uint64_t const desc_v = desc_hi | ((uint64_t)(BLOCK >> 4) << 16);                  // + distance between column blocks
+        // D = f32, A / B = f16, N >> 3, M >> 4; P V reads V with the head dim (its N) contiguous
+        uint32_t const idesc_s = (1u << 4) | ((uint32_t)(BK >> 3) << 17) | ((128u >> 4) << 24);
+        uint32_t const idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(DPAD >> 3) << 17) | ((128u >> 4) << 24);
+        auto issue_s = [&](uint32_t t, uint32_t st) {
+            uint64_t const a = desc_hi | (uint64_t)((sQ + t * TILE) >> 4), b = desc_hi | (uint64_t)((sK + st * TILE) >> 4);
+            uint32_t const d = tmem + t * 128;
+            if (leader) {
+#pragma unroll
+                for (uint32_t i = 0; i < KB * 4; ++i) {
+                    uint64_t const o = (uint64_t)(((i >> 2) * BLOCK + (i & 3) * 32) >> 4);
+                    umma<0>(d, a + o, b + o, idesc_s, i ? 1u : 0u);
+                }
+                umma_commit(s_full + 8 * t);
+            }
+        };
+        auto issue_o = [&](uint32_t t, uint32_t st, bool keep) {
+            uint64_t const b = desc_v | (uint64_t)((sV + st * TILE) >> 4);
+            uint32_t const d = tmem + 256 + t * 128, a = tmem + t * 128;
+            if (leader) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) // 16 keys a product: 8 TMEM columns of P, 16 rows of V
+                    umma_ts(d, a + i * 8, b + (uint64_t)((i * 2048) >> 4), idesc_o, (keep || i) ? 1u : 0u);
+            }
+        };
+        auto commit = [&](uint32_t b) {
+            if (leader) umma_commit(b);
+        };
+        auto wait = [&](uint32_t b, uint32_t parity, uint32_t code) {
+            bool const got = __all_sync(0xffffffffu, wide_wait(p, b, parity, abort_flag, code)) != 0;
+            tc_fence_after();
+            return got;
+        };
+        uint32_t items = 0, tiles = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0}; // tiles and items of each row tile so far
+        bool     ok = true;
+        while (w.left && ok) {
+            uint32_t const n = min(w.kt - w.j, w.left), f0 = first_tile_of<OVH>(w.j), f1 = first_tile_of<OVH>(w.j + n);
+            if (f1 > f0) {
+                uint32_t const start = w.t * TR, count = min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
+                uint32_t const both = count > 128 ? 2 : 1, n_tiles = f1 - f0;
+                ok = wait(q_full, items & 1, 0x31) && wait(k_full + 8 * (tiles & 1), (tiles >> 1) & 1, 0x32);
+                if (!ok) break;
+                for (uint32_t t = 0; t < both; ++t) issue_s(t, tiles & 1);
+                commit(k_empty + 8 * (tiles & 1));
+                if (n_tiles == 1) commit(q_empty);
+                for (uint32_t j = 0; j < n_tiles && ok; ++j) {
+                    uint32_t const at = tiles + j;
+                    for (uint32_t t = 0; t < both; ++t) {
+                        if (j == 0 && !(ok = wait(o_free + 8 * t, (n_o[t] & 1) ^ 1, 0x38))) break;
+                        if (!(ok = wait(p_ready + 8 * t, n_p[t] & 1, 0x34))) break;
+                        ++n_p[t];
+                        if (!(ok = wait(v_full + 8 * (at & 1), (at >> 1) & 1, 0x33))) break;
+                        issue_o(t, at & 1, j != 0);
+                        if (t + 1 == both) commit(v_empty + 8 * (at & 1));
+                        if (j + 1 == n_tiles) {
+                            commit(o_done + 8 * t);
+                            ++n_o[t];
+                        } else {
+                            if (!(ok = wait(k_full + 8 * ((at + 1) & 1), ((at + 1) >> 1) & 1, 0x32))) break;
+                            issue_s(t, (at + 1) & 1);
+                            if (t + 1 == both) {
+                                commit(k_empty + 8 * ((at + 1) & 1));
+                                if (j + 2 == n_tiles) commit(q_empty);
+                            }
+                        }
+                    }
+                }
+                tiles += n_tiles;
+                ++items;
+            }
+            next_item<TR, BK, OVH>(p, w, n);
+        }
+    } else {
+        // ------------------------------------------------------------ softmax: a thread a row
+        uint32_t const t = warp >> 2, r_tile = threadIdx.x & 127;
+        uint32_t const row_s = tmem + t * 128 + ((uint32_t)((warp & 3) * 32) << 16);
+        uint32_t const row_o = row_s + 256;
+        uint32_t       n_s = 0, n_o = 0;
+        bool           ok = true, split = false;
+        while (w.left && ok) {
+            uint32_t const n = min(w.kt - w.j, w.left), f0 = first_tile_of<OVH>(w.j), f1 = first_tile_of<OVH>(w.j + n);
+            uint32_t const start = w.t * TR, count = min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
+            uint32_t const r = t * 128 + r_tile;
+            int const      to = segment_slot(w, n);
+            if (t * 128 < count) {
+                float          m = MMA_NO_KEY, l = 0.f;
+                uint32_t const pr = start + min(r, count - 1), tok = fdivide(pr, p.grp);
+                int const      vis = visible(p, w.s, (int)tok);
+                for (uint32_t j = f0; j < f1; ++j) {
+                    ok = __all_sync(0xffffffffu, wide_wait(p, s_full + 8 * t, n_s & 1, abort_flag, 0x35)) != 0;
+                    if (!ok) break;
+                    ++n_s;
+                    tc_fence_after();
+                    int const  allow = vis - (int)(j * BK); // this row sees the tile's first `allow` keys
+                    bool const mask = __any_sync(0xffffffffu, allow < BK);
+                    float      mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t x[32];
+                        tmem_ld32(row_s + c * 32, x);
+                        if (mask) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (c * 32 + i >= allow) x[i] = 0xff800000u; // -inf
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(x[i]));
+                    }
+                    float const top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                    if (__any_sync(0xffffffffu, top > m + MMA_RESCALE)) {
+                        float const mn = fmaxf(m, top), a = ex2(m - mn);
+                        m = mn;
+                        l *= a;
+                        if (j != f0) {
+#pragma unroll
+                            for (int c = 0; c < DPAD / 32; ++c) {
+                                uint32_t x[32];
+                                tmem_ld32(row_o + c * 32, x);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * a);
+                                tmem_st32(row_o + c * 32, x);
+                            }
+                        }
+                    }
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t x[32], y[16];
+                        tmem_ld32(row_s + c * 32, x);
+                        if (mask) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (c * 32 + i >= allow) x[i] = 0xff800000u;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float const e0 = ex2(fmaf(__uint_as_float(x[2 * i]), p.scale_log2, -m));
+                            float const e1 = ex2(fmaf(__uint_as_float(x[2 * i + 1]), p.scale_log2, -m));
+                            sum[(2 * i) & 3] += e0;
+                            sum[(2 * i + 1) & 3] += e1;
+                            y[i] = pack_h2(e0, e1);
+                        }
+                        tmem_st16(row_s + c * 16, y); // over scores that have been read
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_fence_before();
+                    mbar_arrive(p_ready + 8 * t);
+                }
+                if (!ok) break;
+                if (f1 > f0) {
+                    ok = __all_sync(0xffffffffu, wide_wait(p, o_done + 8 * t, n_o & 1, abort_flag, 0x36)) != 0;
+                    if (!ok) break;
+                    ++n_o;
+                    tc_fence_after();
+                }
+                int const      row = w.s.row0 + (int)tok;
+                uint32_t const head = w.head * p.group + (pr - tok * p.group);
+                uint64_t const at = (uint64_t)row * p.heads + head, part = (uint64_t)(2 * w.worker + max(to, 0)) * TR + r;
+                finish_t       f = {0.f, 0.f, 0.f};
+                if (to < 0 && r < count) {
+                    f = finish(m, l, p.base_lse != nullptr, p.base_lse ? p.base_lse[at] : 0.f);
+                    if (p.lse) p.lse[at] = f.lse;
+                }
+                if (to >= 0 && r < count) p.part_ml[part] = make_float2(m, l);
+#pragma unroll
+                for (int c = 0; c < DPAD / 32; ++c) {
+                    uint32_t x[32];
+                    if (f1 > f0) {
+                        tmem_ld32(row_o + c * 32, x);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] = 0;
+                    }
+                    if (r < count) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            float const v4[4] = {__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])};
+                            if (to < 0) {
+                                if ((uint32_t)(c * 32 + i) < p.d) write_out<__half, 4>(p, row, head, c * 32 + i, v4, f, true);
+                            } else {
+                                *reinterpret_cast<float4*>(p.part_out + part * p.part_d + c * 32 + i) = make_float4(v4[0], v4[1], v4[2], v4[3]);
+                            }
+                        }
+                    }
+                }
+                if (f1 > f0) {
+                    tc_fence_before();
+                    mbar_arrive(o_free + 8 * t);
+                }
+            }
+            if (to == 1) {
+                split = true;
+                if (threadIdx.x == 0) write_meta<TR>(p, w, true);
+            }
+            next_item<TR, BK, OVH>(p, w, n);
+        }
+        if (!split && threadIdx.x == 0) write_meta<TR>(p, w, false);
+    }
+    // ------------------------------------------------------------------ teardown
+    tc_fence_before();
+    __syncthreads();
+    if (ctrl->abort_flag) { // a bounded wait expired: products in flight still read shared memory (bounded: ~1 ms)
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+} // namespace
+} // namespace es
