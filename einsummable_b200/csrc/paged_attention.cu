@@ -147,22 +147,24 @@ template <int NT> int launch_mma(paged_params_t& p, cudaStream_t stream)
     return 2;
 }
 
-template <int DPAD> void launch_wide_as(paged_params_t const& p, cudaStream_t stream)
+template <int DPAD, bool PAGE16> void launch_wide_as(paged_params_t const& p, cudaStream_t stream)
 {
     static bool done[64] = {};
-    allow_smem(paged_wide_kernel<DPAD>, wide_smem_bytes<DPAD>(), done);
-    launch_k(paged_wide_kernel<DPAD>, dim3(WIDE_BLOCKS), dim3(WIDE_THREADS), wide_smem_bytes<DPAD>(), stream, p);
+    allow_smem(paged_wide_kernel<DPAD, PAGE16>, wide_smem_bytes<DPAD>(), done);
+    launch_k(paged_wide_kernel<DPAD, PAGE16>, dim3(WIDE_BLOCKS), dim3(WIDE_THREADS), wide_smem_bytes<DPAD>(), stream, p);
 }
 
 int launch_wide(paged_params_t& p, cudaStream_t stream)
 {
+    bool const page16 = p.page.d % 16 == 0;
     p.part_d = p.d <= 64 ? 64 : 128;
     p.direct = 0;
     p.min_units = 4;
-    if (p.part_d == 64) launch_wide_as<64>(p, stream);
-    else launch_wide_as<128>(p, stream);
+    if (p.part_d == 64) page16 ? launch_wide_as<64, true>(p, stream) : launch_wide_as<64, false>(p, stream);
+    else page16 ? launch_wide_as<128, true>(p, stream) : launch_wide_as<128, false>(p, stream);
     pdl_scope_t scope(true);
-    launch_k(paged_join_kernel<__half, WIDE_TR, 1>, dim3(WIDE_BLOCKS, WIDE_TR / 16), dim3(256), 0, stream, p, 1);
+    if (p.part_d == 64) launch_k(paged_wide_join_kernel<64>, dim3(WIDE_BLOCKS, WIDE_TR / 16), dim3(256), 0, stream, p);
+    else launch_k(paged_wide_join_kernel<128>, dim3(WIDE_BLOCKS, WIDE_TR / 16), dim3(256), 0, stream, p);
     return 2;
 }
 
@@ -175,9 +177,9 @@ int launch_phase(paged_params_t& p, int dtype, bool vec, cudaStream_t stream)
     p.packed_max = 0x7fffffff;
     if (dtype != ES_F16) return launch_simt<float>(p, vec, stream);
     if (!vec || p.d > 128) return launch_simt<__half>(p, vec, stream);
-    bool const     counted = p.prefix_len < 0 && !p.row_offsets;  // one row a sequence
-    uint32_t const most = counted ? p.group : p.rows * p.group;   // packed rows of an item
-    uint32_t const fewest = counted ? p.group : 1;
+    // packed rows of an item: one token's, those of all rows there are, or (row offsets) something in between
+    uint32_t const most = p.prefix_len < 0 && !p.row_offsets ? p.group : p.rows * p.group;
+    uint32_t const fewest = p.row_offsets ? 1 : most;
     int            launches = 0;
     if (fewest <= MMA_MAX_TR) {
         p.packed_max = MMA_MAX_TR;

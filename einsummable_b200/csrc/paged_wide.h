@@ -7,11 +7,13 @@
 // other's are exponentials.  One persistent block an SM, 12 warps:
 //   warps 0-3, 4-7   softmax of tile 0 / 1, a thread a row (= TMEM lane): maximum of the 128 scores, rescaling of
 //                    the accumulator when it has moved by more than 2^8, exponentials (f32; rounded to f16 for
-//                    the product with the values), written as f16 pairs over the scores they came from
+//                    the product with the values), written as f16 pairs over the scores they came from; and the
+//                    copies of the tile's queries, those of the next item as soon as the last scores are there
 //   warp 8           issues the products: S_t = Q_t K^T into TMEM, O_t += P_t V with P_t read from TMEM
-//   warps 9-11       copy the pages: 44 keys a warp, a lane finds a key's page, 16-byte asynchronous copies into
-//                    the 128-byte-swizzled tiles the tensor cores read (any page size: a tile's rows are
-//                    gathered one by one); two stages each for keys and values
+//   warps 9-11       copy the pages into the 128-byte-swizzled tiles the tensor cores read, 16 keys of one page at a
+//                    time (a warp every third 16; one by one where pages are no multiple of 16 tokens, and in the
+//                    sequence's last tile); page numbers are fetched a tile ahead; two stages each for keys and
+//                    values.  (With every row's address sent through a shuffle a tile's 64 KB took 8700 cycles.)
 // TMEM: scores 2 x 128 columns, accumulators 2 x 128.  Products of one thread are done in order, so S_t of the
 // next tile may be issued over P_t as soon as P_t V is, and whoever sees S_t complete knows P_t V to be.
 // Every wait is bounded; on expiry the kernel records 0x31-0x38, lets its copies land, frees TMEM and returns.
@@ -25,7 +27,7 @@ constexpr int      WIDE_TR = 256, WIDE_BK = 128, WIDE_OVH = 2, WIDE_COPY_WARPS =
 constexpr uint64_t WIDE_WAIT_LIMIT_CYCLES = 4000000000ull; // ~2 s at 2 GHz
 
 struct wide_ctrl_t {
-    uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], o_free[2];
+    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], o_free[2];
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
@@ -56,6 +58,20 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
 }
+// 32 columns of this thread's lane, there after tcgen05.wait::ld
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, uint32_t const (&r)[16])
 {
     asm volatile(
@@ -71,7 +87,7 @@ template <int DPAD> constexpr uint32_t wide_smem_bytes()
     return (2 + 2 + 2) * (DPAD / 64) * 16384 + (uint32_t)sizeof(wide_ctrl_t) + 1024;
 }
 
-template <int DPAD>
+template <int DPAD, bool PAGE16> // PAGE16: pages are a multiple of 16 tokens
 __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __grid_constant__ paged_params_t p)
 {
     constexpr int      TR = WIDE_TR, BK = WIDE_BK, OVH = WIDE_OVH;
@@ -83,14 +99,13 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
     volatile uint32_t* abort_flag = &ctrl->abort_flag;
     uint32_t const     sQ = smem_u32(smem), sK = sQ + 2 * TILE, sV = sK + 2 * TILE; // two tiles each
     uint32_t const     bars = smem_u32(ctrl);
-    uint32_t const     q_full = bars, q_empty = bars + 8; // in the order of wide_ctrl_t
-    uint32_t const     k_full = q_empty + 8, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16, s_full = v_empty + 16,
+    // in the order of wide_ctrl_t
+    uint32_t const     q_full = bars, k_full = q_full + 16, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16, s_full = v_empty + 16,
                    p_ready = s_full + 16, o_done = p_ready + 16, o_free = o_done + 16;
     int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        mbar_init(q_full, WIDE_COPY_WARPS * 32);
-        mbar_init(q_empty, 1);
         for (int i = 0; i < 2; ++i) {
+            mbar_init(q_full + 8 * i, 128);
             mbar_init(k_full + 8 * i, WIDE_COPY_WARPS * 32);
             mbar_init(k_empty + 8 * i, 1);
             mbar_init(v_full + 8 * i, WIDE_COPY_WARPS * 32);
@@ -120,100 +135,100 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
     find_work<TR, BK, OVH, WIDE_THREADS, 1>(p, w, sched);
 
     if (warp >= 9) {
-        // ------------------------------------------------------------ copies
-        constexpr int  CH = DPAD / 8, ROWS_AT = 32 / CH;
+        // ------------------------------------------------------------ copies of keys and values
+        constexpr int  CH = DPAD / 8, ROWS_AT = 32 / CH, STEPS = 16 / ROWS_AT;
         int const      lw = warp - 9, c_row = lane / CH, c_chunk = lane % CH;
         bool const     c_on = (uint32_t)c_chunk * 8 < p.d;
-        uint32_t const c_col = (uint32_t)(c_chunk >> 3) * BLOCK, cc = c_chunk & 7;
-        // groups of copies in flight, oldest first: the barrier that each completes
-        uint32_t pend[3];
-        int      n_pend = 0;
-        auto     signal = [&](uint32_t b) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(b);
-        };
-        auto flush = [&]() {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            for (int i = 0; i < n_pend; ++i) signal(pend[i]);
-            n_pend = 0;
-        };
-        auto commit = [&](uint32_t b) {
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (n_pend == 2) {
-                asm volatile("cp.async.wait_group 2;" ::: "memory");
-                signal(pend[0]);
-                pend[0] = pend[1];
-                n_pend = 1;
-            }
-            pend[n_pend++] = b;
-        };
+        // chunk c of row r lies in block c / 8 at chunk (c % 8) ^ (r % 8)
+        uint32_t const c_dst = (uint32_t)(c_chunk >> 3) * BLOCK + c_row * 128 + (((c_chunk & 7) ^ c_row) << 4);
+        uint32_t const k_step = (uint32_t)p.k_stride[1] * ROWS_AT, v_step = (uint32_t)p.v_stride[1] * ROWS_AT;
+        // the barrier is arrived at when this thread's copies so far have landed; nobody waits here for them
+        // (whoever waits for the barrier orders what they wrote before the tensor cores' reads)
+        auto commit = [&](uint32_t b) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(b) : "memory"); };
         auto acquire = [&](uint32_t b, uint32_t parity) { // a tile that the products no longer read
-            if (__all_sync(0xffffffffu, mbar_try_wait(b, parity))) return true;
-            flush(); // what has been copied may be what they wait for
             return __all_sync(0xffffffffu, wide_wait(p, b, parity, abort_flag, 0x37)) != 0;
         };
-        uint32_t items = 0, tiles = 0;
+        uint32_t tiles = 0;
         bool     ok = true;
         while (w.left && ok) {
             uint32_t const n = min(w.kt - w.j, w.left), f0 = first_tile_of<OVH>(w.j), f1 = first_tile_of<OVH>(w.j + n);
-            if (f1 > f0) {
-                uint32_t const start = w.t * TR, count = min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
-                ok = acquire(q_empty, (items & 1) ^ 1);
-                if (!ok) break;
-                for (uint32_t r = lw * ROWS_AT + c_row; r < (count + 127) / 128 * 128; r += WIDE_COPY_WARPS * ROWS_AT) {
-                    uint32_t const pr = min(start + r, start + count - 1), tok = fdivide(pr, p.grp);
-                    __half const*  src = static_cast<__half const*>(p.q) + (int64_t)(w.s.row0 + (int)tok) * p.q_stride[0] +
-                                        (int64_t)(w.head * p.group + (pr - tok * p.group)) * p.q_stride[1] + c_chunk * 8;
-                    uint32_t const dst = sQ + (r >> 7) * TILE + c_col + (r & 127) * 128 + ((cc ^ (r & 7)) << 4);
-                    if (c_on) copy16(dst, src, r < count);
-                }
-                commit(q_full);
-                ++items;
-                for (uint32_t j = f0; j < f1 && ok; ++j, ++tiles) {
-                    // where this warp's keys lie: lane x has keys x and 32 + x of its range
-                    uint32_t const range = lw * 44, range_n = min(44u, 128u - range);
-                    int64_t        ko[2] = {0, 0}, vo[2] = {0, 0};
-                    unsigned       ons[2];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        uint32_t const at = lane + 32 * x, key = j * BK + range + at;
-                        bool           on = at < range_n && key < (uint32_t)w.s.len;
-                        if (on) {
-                            uint32_t const pi = fdivide(key, p.page), slot = key - pi * p.page.d;
-                            uint32_t const page = (uint32_t)w.s.table[pi];
-                            on = page < p.n_pages;
-                            if (!on) report(p, PAGED_BAD_PAGE);
-                            ko[x] = (int64_t)page * p.k_stride[0] + (int64_t)slot * p.k_stride[1] + (int64_t)w.head * p.k_stride[2];
-                            vo[x] = (int64_t)page * p.v_stride[0] + (int64_t)slot * p.v_stride[1] + (int64_t)w.head * p.v_stride[2];
-                        }
-                        ons[x] = __ballot_sync(0xffffffffu, on);
+            // lane g: the page of this tile's keys 16 g ..
+            auto page_of = [&](uint32_t j) {
+                uint32_t const key = j * BK + lane * 16;
+                return PAGE16 && lane < BK / 16 && key < (uint32_t)w.s.len ? (uint32_t)w.s.table[fdivide(key, p.page)] : 0u;
+            };
+            uint32_t next_page = f1 > f0 ? page_of(f0) : 0u;
+            for (uint32_t j = f0; j < f1 && ok; ++j, ++tiles) {
+                uint32_t page = next_page;
+                if (j + 1 < f1) next_page = page_of(j + 1);
+                uint32_t const st = tiles & 1, par = ((tiles >> 1) & 1) ^ 1;
+                uint32_t const to_k = sK + st * TILE, to_v = sV + st * TILE;
+                if (PAGE16 && (j + 1) * BK <= (uint32_t)w.s.len) {
+                    if (page >= p.n_pages) {
+                        report(p, PAGED_BAD_PAGE); // (reads page 0, which is there)
+                        page = 0;
                     }
-                    uint32_t const st = tiles & 1, par = ((tiles >> 1) & 1) ^ 1;
-                    auto copy_tile = [&](uint32_t dst, void const* base, int64_t const (&off)[2]) {
+                    uint32_t const key = j * BK + lane * 16;
+                    uint32_t const slot = lane < BK / 16 ? key - fdivide(key, p.page) * p.page.d : 0u;
+                    auto copy_tile = [&](uint32_t to, void const* base, int64_t const (&stride)[3], uint32_t step) {
 #pragma unroll
-                        for (int x = 0; x < 2; ++x)
-#pragma unroll 4
-                            for (int i = 0; i < 32 / ROWS_AT; ++i) {
-                                uint32_t const r = c_row + i * ROWS_AT, row = range + 32 * x + r;
-                                if (32 * x + i * ROWS_AT >= range_n) break; // (ranges are multiples of 4 rows)
-                                int64_t const at = __shfl_sync(0xffffffffu, off[x], r);
-                                bool const    live = (ons[x] >> r) & 1;
-                                if (c_on)
-                                    copy16(dst + c_col + row * 128 + ((cc ^ (row & 7)) << 4),
-                                           live ? (void const*)(static_cast<__half const*>(base) + at + c_chunk * 8) : base, live);
+                        for (int x = 0; x < 3; ++x) {
+                            uint32_t const g = lw + WIDE_COPY_WARPS * x;
+                            if (g < BK / 16) {
+                                uint32_t const pg = __shfl_sync(0xffffffffu, page, g), sl = __shfl_sync(0xffffffffu, slot, g);
+                                __half const*  src = static_cast<__half const*>(base) + (int64_t)pg * stride[0] +
+                                                    (int64_t)(sl + c_row) * stride[1] + (int64_t)w.head * stride[2] + c_chunk * 8;
+                                uint32_t const dst = to + g * 2048;
+                                if (c_on) {
+#pragma unroll
+                                    for (int i = 0; i < STEPS; ++i)
+                                        copy16(dst + (c_dst ^ (((i * ROWS_AT) & 7) << 4)) + i * ROWS_AT * 128, src + (uint64_t)step * i, true);
+                                }
                             }
+                        }
                     };
                     if (!(ok = acquire(k_empty + 8 * st, par))) break;
-                    copy_tile(sK + st * TILE, p.k, ko);
+                    copy_tile(to_k, p.k, p.k_stride, k_step);
                     commit(k_full + 8 * st);
                     if (!(ok = acquire(v_empty + 8 * st, par))) break;
-                    copy_tile(sV + st * TILE, p.v, vo);
+                    copy_tile(to_v, p.v, p.v_stride, v_step);
+                    commit(v_full + 8 * st);
+                } else {
+                    if (!(ok = acquire(k_empty + 8 * st, par))) break;
+                    if (!(ok = acquire(v_empty + 8 * st, par))) break;
+#pragma unroll 1
+                    for (uint32_t g = lw; g < BK / 16; g += WIDE_COPY_WARPS) { // lane r < 16 finds key r of 16
+                        uint32_t const key = j * BK + g * 16 + lane;
+                        int64_t        ko = 0, vo = 0;
+                        bool           on = lane < 16 && key < (uint32_t)w.s.len;
+                        if (on) {
+                            uint32_t const pi = fdivide(key, p.page), slot = key - pi * p.page.d;
+                            uint32_t const pg = (uint32_t)w.s.table[pi];
+                            on = pg < p.n_pages;
+                            if (!on) report(p, PAGED_BAD_PAGE);
+                            ko = (int64_t)pg * p.k_stride[0] + (int64_t)slot * p.k_stride[1] + (int64_t)w.head * p.k_stride[2];
+                            vo = (int64_t)pg * p.v_stride[0] + (int64_t)slot * p.v_stride[1] + (int64_t)w.head * p.v_stride[2];
+                        }
+                        unsigned const ons = __ballot_sync(0xffffffffu, on);
+#pragma unroll 2
+                        for (int i = 0; i < STEPS; ++i) {
+                            uint32_t const r = c_row + i * ROWS_AT;
+                            int64_t const  k_at = __shfl_sync(0xffffffffu, ko, r), v_at = __shfl_sync(0xffffffffu, vo, r);
+                            bool const     live = (ons >> r) & 1;
+                            uint32_t const dst = (c_dst ^ (((i * ROWS_AT) & 7) << 4)) + i * ROWS_AT * 128 + g * 2048;
+                            if (c_on) {
+                                copy16(to_k + dst, live ? (void const*)(static_cast<__half const*>(p.k) + k_at + c_chunk * 8) : p.k, live);
+                                copy16(to_v + dst, live ? (void const*)(static_cast<__half const*>(p.v) + v_at + c_chunk * 8) : p.v, live);
+                            }
+                        }
+                    }
+                    commit(k_full + 8 * st);
                     commit(v_full + 8 * st);
                 }
             }
             next_item<TR, BK, OVH>(p, w, n);
         }
-        flush();
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == 8) {
         // ------------------------------------------------------------ products (the whole warp; one lane issues)
         bool leader;
@@ -253,21 +268,22 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
         };
         auto wait = [&](uint32_t b, uint32_t parity, uint32_t code) {
             bool const got = __all_sync(0xffffffffu, wide_wait(p, b, parity, abort_flag, code)) != 0;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the copies are ordinary writes, the products' reads are not
             tc_fence_after();
             return got;
         };
-        uint32_t items = 0, tiles = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0}; // tiles and items of each row tile so far
+        uint32_t tiles = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0}; // tiles and items of each row tile so far
         bool     ok = true;
         while (w.left && ok) {
             uint32_t const n = min(w.kt - w.j, w.left), f0 = first_tile_of<OVH>(w.j), f1 = first_tile_of<OVH>(w.j + n);
             if (f1 > f0) {
                 uint32_t const start = w.t * TR, count = min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
                 uint32_t const both = count > 128 ? 2 : 1, n_tiles = f1 - f0;
-                ok = wait(q_full, items & 1, 0x31) && wait(k_full + 8 * (tiles & 1), (tiles >> 1) & 1, 0x32);
+                ok = wait(k_full + 8 * (tiles & 1), (tiles >> 1) & 1, 0x32);
+                for (uint32_t t = 0; t < both && ok; ++t)
+                    if ((ok = wait(q_full + 8 * t, n_o[t] & 1, 0x31))) issue_s(t, tiles & 1);
                 if (!ok) break;
-                for (uint32_t t = 0; t < both; ++t) issue_s(t, tiles & 1);
                 commit(k_empty + 8 * (tiles & 1));
-                if (n_tiles == 1) commit(q_empty);
                 for (uint32_t j = 0; j < n_tiles && ok; ++j) {
                     uint32_t const at = tiles + j;
                     for (uint32_t t = 0; t < both; ++t) {
@@ -283,15 +299,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                         } else {
                             if (!(ok = wait(k_full + 8 * ((at + 1) & 1), ((at + 1) >> 1) & 1, 0x32))) break;
                             issue_s(t, (at + 1) & 1);
-                            if (t + 1 == both) {
-                                commit(k_empty + 8 * ((at + 1) & 1));
-                                if (j + 2 == n_tiles) commit(q_empty);
-                            }
+                            if (t + 1 == both) commit(k_empty + 8 * ((at + 1) & 1));
                         }
                     }
                 }
                 tiles += n_tiles;
-                ++items;
             }
             next_item<TR, BK, OVH>(p, w, n);
         }
@@ -302,11 +314,40 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
         uint32_t const row_o = row_s + 256;
         uint32_t       n_s = 0, n_o = 0;
         bool           ok = true, split = false;
+        // this warp's 32 query rows of an item's tile t (none if the item has no key tile here); tell_q follows
+        auto load_q = [&](work_t const& x) -> bool {
+            if (x.left == 0) return false;
+            uint32_t const n = min(x.kt - x.j, x.left), start = x.t * TR, count = min((uint32_t)TR, (uint32_t)x.s.n * p.group - start);
+            if (first_tile_of<OVH>(x.j + n) == first_tile_of<OVH>(x.j) || t * 128 >= count) return false;
+            constexpr int  CH = DPAD / 8, ROWS_AT = 32 / CH;
+            uint32_t const first = t * 128 + (warp & 3) * 32;
+            uint32_t const pr = start + min(first + lane, count - 1), tok = fdivide(pr, p.grp);
+            int64_t const  mine = (int64_t)(x.s.row0 + (int)tok) * p.q_stride[0] + (int64_t)(x.head * p.group + (pr - tok * p.group)) * p.q_stride[1];
+            uint32_t const c_row = lane / CH, c = lane % CH;
+            __half const*  q = static_cast<__half const*>(p.q) + c * 8;
+#pragma unroll 4
+            for (int i = 0; i < 32 / ROWS_AT; ++i) {
+                uint32_t const r = c_row + i * ROWS_AT, row = (first & 127) + r;
+                int64_t const  at = __shfl_sync(0xffffffffu, mine, r);
+                if (c * 8 < p.d) copy16(sQ + t * TILE + (c >> 3) * BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4), q + at, first + r < count);
+            }
+            return true;
+        };
+        auto tell_q = [&]() {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(q_full + 8 * t);
+        };
+        if (load_q(w)) tell_q();
         while (w.left && ok) {
             uint32_t const n = min(w.kt - w.j, w.left), f0 = first_tile_of<OVH>(w.j), f1 = first_tile_of<OVH>(w.j + n);
             uint32_t const start = w.t * TR, count = min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
             uint32_t const r = t * 128 + r_tile;
             int const      to = segment_slot(w, n);
+            work_t         wn = w;
+            next_item<TR, BK, OVH>(p, wn, n);
+            bool const here = t * 128 < count && f1 > f0; // this warp has rows and keys in the item
+            if (!here && load_q(wn)) tell_q();
             if (t * 128 < count) {
                 float          m = MMA_NO_KEY, l = 0.f;
                 uint32_t const pr = start + min(r, count - 1), tok = fdivide(pr, p.grp);
@@ -316,61 +357,59 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     if (!ok) break;
                     ++n_s;
                     tc_fence_after();
+                    // every product with this item's queries is done: the next item's may come
+                    bool const last = j + 1 == f1, more = last && load_q(wn);
                     int const  allow = vis - (int)(j * BK); // this row sees the tile's first `allow` keys
-                    bool const mask = __any_sync(0xffffffffu, allow < BK);
-                    float      mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    uint32_t   x[BK];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t x[32];
-                        tmem_ld32(row_s + c * 32, x);
-                        if (mask) {
+                    for (int c = 0; c < 4; ++c) tmem_ld32_async(row_s + c * 32, x + c * 32);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (__any_sync(0xffffffffu, allow < BK)) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (c * 32 + i >= allow) x[i] = 0xff800000u; // -inf
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(x[i]));
+                        for (int i = 0; i < BK; ++i)
+                            if (i >= allow) x[i] = 0xff800000u; // -inf
                     }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < BK; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(x[i]));
                     float const top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-                    if (__any_sync(0xffffffffu, top > m + MMA_RESCALE)) {
-                        float const mn = fmaxf(m, top), a = ex2(m - mn);
+                    float       a = 1.f;
+                    bool const  move = __any_sync(0xffffffffu, top > m + MMA_RESCALE);
+                    if (move) {
+                        float const mn = fmaxf(m, top);
+                        a = ex2(m - mn);
                         m = mn;
                         l *= a;
-                        if (j != f0) {
-#pragma unroll
-                            for (int c = 0; c < DPAD / 32; ++c) {
-                                uint32_t x[32];
-                                tmem_ld32(row_o + c * 32, x);
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * a);
-                                tmem_st32(row_o + c * 32, x);
-                            }
-                        }
                     }
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t x[32], y[16];
-                        tmem_ld32(row_s + c * 32, x);
-                        if (mask) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (c * 32 + i >= allow) x[i] = 0xff800000u;
-                        }
+                        uint32_t y[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            float const e0 = ex2(fmaf(__uint_as_float(x[2 * i]), p.scale_log2, -m));
-                            float const e1 = ex2(fmaf(__uint_as_float(x[2 * i + 1]), p.scale_log2, -m));
+                            float const e0 = ex2(fmaf(__uint_as_float(x[c * 32 + 2 * i]), p.scale_log2, -m));
+                            float const e1 = ex2(fmaf(__uint_as_float(x[c * 32 + 2 * i + 1]), p.scale_log2, -m));
                             sum[(2 * i) & 3] += e0;
                             sum[(2 * i + 1) & 3] += e1;
                             y[i] = pack_h2(e0, e1);
                         }
-                        tmem_st16(row_s + c * 16, y); // over scores that have been read
+                        tmem_st16(row_s + c * 16, y); // over the scores, which have been read
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    if (move && j != f0) {
+#pragma unroll 1
+                        for (int c = 0; c < DPAD / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_ld32(row_o + c * 32, o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+                            tmem_st32(row_o + c * 32, o);
+                        }
+                    }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                     mbar_arrive(p_ready + 8 * t);
+                    if (more) tell_q();
                 }
                 if (!ok) break;
                 if (f1 > f0) {
@@ -388,7 +427,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     if (p.lse) p.lse[at] = f.lse;
                 }
                 if (to >= 0 && r < count) p.part_ml[part] = make_float2(m, l);
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < DPAD / 32; ++c) {
                     uint32_t x[32];
                     if (f1 > f0) {
@@ -404,7 +443,9 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                             if (to < 0) {
                                 if ((uint32_t)(c * 32 + i) < p.d) write_out<__half, 4>(p, row, head, c * 32 + i, v4, f, true);
                             } else {
-                                *reinterpret_cast<float4*>(p.part_out + part * p.part_d + c * 32 + i) = make_float4(v4[0], v4[1], v4[2], v4[3]);
+                                // four elements of 256 rows, then the next four: a warp's store is one run of 512 bytes
+                                *reinterpret_cast<float4*>(p.part_out + (uint64_t)(2 * w.worker + to) * TR * DPAD + ((c * 8 + i / 4) * TR + r) * 4) =
+                                    make_float4(v4[0], v4[1], v4[2], v4[3]);
                             }
                         }
                     }
@@ -418,7 +459,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                 split = true;
                 if (threadIdx.x == 0) write_meta<TR>(p, w, true);
             }
-            next_item<TR, BK, OVH>(p, w, n);
+            w = wn;
         }
         if (!split && threadIdx.x == 0) write_meta<TR>(p, w, false);
     }
@@ -432,6 +473,81 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
     if (warp == 8) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// Joins the partial results of the items that crossed shares (see paged_join_kernel): block x the item that
+// starts last in share x, block y 16 of its rows; thread (row, 4 elements), a half warp reads 16 rows' runs.  The
+// rows leave through shared memory in 16-byte pieces.
+template <int DPAD> __global__ void __launch_bounds__(256) paged_wide_join_kernel(const __grid_constant__ paged_params_t p)
+{
+    constexpr int    TR = WIDE_TR, CH = DPAD / 64; // chunks of 64 elements, 4 a thread
+    __shared__ float so[16][DPAD + 4];
+    ES_PDL_PROLOGUE();
+    int4 const     m0 = p.meta[2 * blockIdx.x];
+    uint32_t const r0 = blockIdx.y * 16;
+    if (r0 >= (uint32_t)m0.x) return;
+    int const      first = (int)blockIdx.x, n = p.meta[2 * blockIdx.x + 1].x - first + 1;
+    uint32_t const rows = min((uint32_t)m0.x - r0, 16u), rr = threadIdx.x & 15, c4 = threadIdx.x >> 4;
+    uint32_t const r = r0 + min(rr, rows - 1);
+    auto  slot = [&](int i) { return (uint64_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * TR; };
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        float2 const ml = p.part_ml[slot(i) + r];
+        top = fmaxf(top, ml.y == 0.f ? -INFINITY : ml.x);
+    }
+    float o[CH][4] = {}, l = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        float2 const ml = p.part_ml[slot(i) + r];
+        float const  wgt = ml.y == 0.f ? 0.f : ex2(ml.x - top);
+        l = fmaf(ml.y, wgt, l);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            float4 const x = *reinterpret_cast<float4 const*>(p.part_out + slot(i) * DPAD + ((c * 16 + c4) * TR + r) * 4);
+            o[c][0] = fmaf(x.x, wgt, o[c][0]);
+            o[c][1] = fmaf(x.y, wgt, o[c][1]);
+            o[c][2] = fmaf(x.z, wgt, o[c][2]);
+            o[c][3] = fmaf(x.w, wgt, o[c][3]);
+        }
+    }
+    auto place = [&](uint32_t at_row, int& row, uint32_t& head) {
+        uint32_t const pr = (uint32_t)m0.z + at_row, tok = fdivide(pr, p.grp);
+        row = m0.y + (int)tok;
+        head = (uint32_t)m0.w * p.group + (pr - tok * p.group);
+    };
+    int      row;
+    uint32_t head;
+    place(r, row, head);
+    uint64_t const at = (uint64_t)row * p.heads + head;
+    finish_t const f = finish(top, l, p.base_lse != nullptr, p.base_lse ? p.base_lse[at] : 0.f);
+    if (p.lse && c4 == 0 && rr < rows) p.lse[at] = f.lse;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        uint32_t const e = (c * 16 + c4) * 4;
+        float          v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] = f.wa == 0.f ? 0.f : o[c][k] * f.wa;
+            if (f.wb != 0.f && e + k < p.d) v[k] = fmaf(p.base_out[at * p.d + e + k], f.wb, v[k]);
+        }
+        *reinterpret_cast<float4*>(&so[rr][e]) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+    __syncthreads();
+    uint32_t const wr = threadIdx.x >> 4;
+    if (wr >= rows) return;
+    place(r0 + wr, row, head);
+    for (uint32_t e = (threadIdx.x & 15) * 8; e < p.d; e += 128) { // (the head dim is a multiple of 8)
+        float4 const a = *reinterpret_cast<float4 const*>(&so[wr][e]), b = *reinterpret_cast<float4 const*>(&so[wr][e + 4]);
+        if (p.out_f32) {
+            float* d = static_cast<float*>(p.out) + ((uint64_t)row * p.heads + head) * p.d + e;
+            *reinterpret_cast<float4*>(d) = a;
+            *reinterpret_cast<float4*>(d + 4) = b;
+        } else {
+            __half* d = static_cast<__half*>(p.out) + (int64_t)row * p.out_stride[0] + (int64_t)head * p.out_stride[1] + e;
+            *reinterpret_cast<uint4*>(d) = make_uint4(pack_h2(a.x, a.y), pack_h2(a.z, a.w), pack_h2(b.x, b.y), pack_h2(b.z, b.w));
+        }
     }
 }
 
