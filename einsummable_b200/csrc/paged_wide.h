@@ -23,7 +23,7 @@
 namespace es {
 namespace {
 
-constexpr int      WIDE_TR = 256, WIDE_BK = 128, WIDE_OVH = 2, WIDE_COPY_WARPS = 3, WIDE_THREADS = (9 + WIDE_COPY_WARPS) * 32;
+constexpr int      WIDE_TR = 256, WIDE_BK = 128, WIDE_OVH = 4, WIDE_COPY_WARPS = 3, WIDE_THREADS = (9 + WIDE_COPY_WARPS) * 32;
 constexpr uint64_t WIDE_WAIT_LIMIT_CYCLES = 4000000000ull; // ~2 s at 2 GHz
 
 struct wide_ctrl_t {
@@ -82,9 +82,44 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, uint32_t const (&r)[16
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_wait_ld()
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// two f32 at a time
+__device__ __forceinline__ uint64_t pack2(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t x, float& lo, float& hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+constexpr uint32_t WIDE_STAGE_BYTES = 8 * 2048; // results on their way out: 32 rows of 32 f16 a warp
 template <int DPAD> constexpr uint32_t wide_smem_bytes()
 {
-    return (2 + 2 + 2) * (DPAD / 64) * 16384 + (uint32_t)sizeof(wide_ctrl_t) + 1024;
+    return 6 * (DPAD / 64) * 16384 + WIDE_STAGE_BYTES + (uint32_t)sizeof(wide_ctrl_t) + 1024;
 }
 
 template <int DPAD, bool PAGE16> // PAGE16: pages are a multiple of 16 tokens
@@ -95,7 +130,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
     __shared__ sched_smem_t<WIDE_THREADS, 1> sched;
     extern __shared__ uint8_t                smem_wide[];
     uint8_t* const     smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_wide) + 1023) & ~uintptr_t(1023));
-    wide_ctrl_t* const ctrl = reinterpret_cast<wide_ctrl_t*>(smem + 6 * TILE);
+    wide_ctrl_t* const ctrl = reinterpret_cast<wide_ctrl_t*>(smem + 6 * TILE + WIDE_STAGE_BYTES);
     volatile uint32_t* abort_flag = &ctrl->abort_flag;
     uint32_t const     sQ = smem_u32(smem), sK = sQ + 2 * TILE, sV = sK + 2 * TILE; // two tiles each
     uint32_t const     bars = smem_u32(ctrl);
@@ -268,7 +303,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
         };
         auto wait = [&](uint32_t b, uint32_t parity, uint32_t code) {
             bool const got = __all_sync(0xffffffffu, wide_wait(p, b, parity, abort_flag, code)) != 0;
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the copies are ordinary writes, the products' reads are not
+            // keys and values: the copies are ordinary writes, the products' reads are not
+            if (code == 0x32 || code == 0x33) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc_fence_after();
             return got;
         };
@@ -288,16 +324,16 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     uint32_t const at = tiles + j;
                     for (uint32_t t = 0; t < both; ++t) {
                         if (j == 0 && !(ok = wait(o_free + 8 * t, (n_o[t] & 1) ^ 1, 0x38))) break;
+                        if (t == 0 && !(ok = wait(v_full + 8 * (at & 1), (at >> 1) & 1, 0x33))) break;
                         if (!(ok = wait(p_ready + 8 * t, n_p[t] & 1, 0x34))) break;
                         ++n_p[t];
-                        if (!(ok = wait(v_full + 8 * (at & 1), (at >> 1) & 1, 0x33))) break;
                         issue_o(t, at & 1, j != 0);
                         if (t + 1 == both) commit(v_empty + 8 * (at & 1));
                         if (j + 1 == n_tiles) {
                             commit(o_done + 8 * t);
                             ++n_o[t];
                         } else {
-                            if (!(ok = wait(k_full + 8 * ((at + 1) & 1), ((at + 1) >> 1) & 1, 0x32))) break;
+                            if (t == 0 && !(ok = wait(k_full + 8 * ((at + 1) & 1), ((at + 1) >> 1) & 1, 0x32))) break;
                             issue_s(t, (at + 1) & 1);
                             if (t + 1 == both) commit(k_empty + 8 * ((at + 1) & 1));
                         }
@@ -344,10 +380,13 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
             uint32_t const start = w.t * TR, count = min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
             uint32_t const r = t * 128 + r_tile;
             int const      to = segment_slot(w, n);
-            work_t         wn = w;
-            next_item<TR, BK, OVH>(p, wn, n);
+            auto load_next_q = [&]() { // (not kept: registers)
+                work_t wn = w;
+                next_item<TR, BK, OVH>(p, wn, n);
+                return load_q(wn);
+            };
             bool const here = t * 128 < count && f1 > f0; // this warp has rows and keys in the item
-            if (!here && load_q(wn)) tell_q();
+            if (!here && load_next_q()) tell_q();
             if (t * 128 < count) {
                 float          m = MMA_NO_KEY, l = 0.f;
                 uint32_t const pr = start + min(r, count - 1), tok = fdivide(pr, p.grp);
@@ -358,57 +397,88 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     ++n_s;
                     tc_fence_after();
                     // every product with this item's queries is done: the next item's may come
-                    bool const last = j + 1 == f1, more = last && load_q(wn);
+                    bool const more = j + 1 == f1 && load_next_q();
                     int const  allow = vis - (int)(j * BK); // this row sees the tile's first `allow` keys
-                    uint32_t   x[BK];
+                    bool const mask = __any_sync(0xffffffffu, allow < BK);
+                    // Scores are read 64 at a time (128 at once do not fit beside the rest): the maximum of the second
+                    // half, then of the first, which stays for its exponentials; P of the first half may then lie over
+                    // it, and the second half is read again.
+                    auto hide = [&](uint32_t (&v)[32], int first) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32_async(row_s + c * 32, x + c * 32);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (__any_sync(0xffffffffu, allow < BK)) {
-#pragma unroll
-                        for (int i = 0; i < BK; ++i)
-                            if (i >= allow) x[i] = 0xff800000u; // -inf
-                    }
+                        for (int i = 0; i < 32; ++i)
+                            if (first + i >= allow) v[i] = 0xff800000u; // -inf
+                    };
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    auto  largest = [&](uint32_t (&v)[32]) {
 #pragma unroll
-                    for (int i = 0; i < BK; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(x[i]));
-                    float const top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-                    float       a = 1.f;
-                    bool const  move = __any_sync(0xffffffffu, top > m + MMA_RESCALE);
-                    if (move) {
-                        float const mn = fmaxf(m, top);
-                        a = ex2(m - mn);
+                        for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                    };
+                    uint32_t x0[32], x1[32];
+                    tmem_ld32_async(row_s + 64, x0);
+                    tmem_ld32_async(row_s + 96, x1);
+                    tmem_wait_ld();
+                    if (mask) {
+                        hide(x0, 64);
+                        hide(x1, 96);
+                    }
+                    largest(x0);
+                    largest(x1);
+                    tmem_ld32_async(row_s, x0);
+                    tmem_ld32_async(row_s + 32, x1);
+                    tmem_wait_ld();
+                    if (mask) {
+                        hide(x0, 0);
+                        hide(x1, 32);
+                    }
+                    largest(x0);
+                    largest(x1);
+                    float const top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;
+                    if (__any_sync(0xffffffffu, top > m + MMA_RESCALE)) {
+                        float const mn = fmaxf(m, top), a = ex2(m - mn);
                         m = mn;
                         l *= a;
-                    }
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                        if (j != f0) {
+#pragma unroll 1
+                            for (int c = 0; c < DPAD / 32; ++c) {
+                                uint32_t o[32];
+                                tmem_ld32(row_o + c * 32, o);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+                                tmem_st32(row_o + c * 32, o);
+                            }
+                        }
+                    }
+                    uint64_t const scale2 = pack2(p.scale_log2, p.scale_log2), m2 = pack2(-m, -m);
+                    uint64_t       sum[2] = {0, 0};
+                    auto exponentials = [&](uint32_t (&v)[32], int c) { // of 32 scores, into P's columns 16 c ..
                         uint32_t y[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            float const e0 = ex2(fmaf(__uint_as_float(x[c * 32 + 2 * i]), p.scale_log2, -m));
-                            float const e1 = ex2(fmaf(__uint_as_float(x[c * 32 + 2 * i + 1]), p.scale_log2, -m));
-                            sum[(2 * i) & 3] += e0;
-                            sum[(2 * i + 1) & 3] += e1;
+                            float e0, e1;
+                            unpack2(fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, m2), e0, e1);
+                            e0 = ex2(e0);
+                            e1 = ex2(e1);
+                            sum[i & 1] = add2(sum[i & 1], pack2(e0, e1));
                             y[i] = pack_h2(e0, e1);
                         }
-                        tmem_st16(row_s + c * 16, y); // over the scores, which have been read
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    if (move && j != f0) {
-#pragma unroll 1
-                        for (int c = 0; c < DPAD / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_ld32(row_o + c * 32, o);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-                            tmem_st32(row_o + c * 32, o);
-                        }
-                    }
+                        tmem_st16(row_s + c * 16, y);
+                    };
+                    exponentials(x0, 0);
+                    tmem_ld32_async(row_s + 64, x0);
+                    exponentials(x1, 1);
+                    tmem_wait_ld();
+                    tmem_ld32_async(row_s + 96, x1);
+                    if (mask) hide(x0, 64);
+                    exponentials(x0, 2);
+                    tmem_wait_ld();
+                    if (mask) hide(x1, 96);
+                    exponentials(x1, 3);
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                     mbar_arrive(p_ready + 8 * t);
+                    float s0, s1;
+                    unpack2(add2(sum[0], sum[1]), s0, s1);
+                    l += s0 + s1;
                     if (more) tell_q();
                 }
                 if (!ok) break;
@@ -427,6 +497,19 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     if (p.lse) p.lse[at] = f.lse;
                 }
                 if (to >= 0 && r < count) p.part_ml[part] = make_float2(m, l);
+                bool const staged = to < 0 && !p.out_f32; // f16 rows go out through shared memory
+                __half*    dst[4] = {};                   // row (lane / 4) + 8 i of the warp's 32, elements 8 (lane % 4) ..
+                if (staged) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t const rw = t * 128 + (warp & 3) * 32 + (lane >> 2) + 8 * i;
+                        uint32_t const q = start + min(rw, count - 1), qt = fdivide(q, p.grp);
+                        if (rw < count)
+                            dst[i] = static_cast<__half*>(p.out) + (int64_t)(w.s.row0 + (int)qt) * p.out_stride[0] +
+                                     (int64_t)(w.head * p.group + (q - qt * p.group)) * p.out_stride[1] + (lane & 3) * 8;
+                    }
+                }
+                uint32_t const stage = sQ + 6 * TILE + warp * 2048;
 #pragma unroll 1
                 for (int c = 0; c < DPAD / 32; ++c) {
                     uint32_t x[32];
@@ -436,7 +519,39 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
 #pragma unroll
                         for (int i = 0; i < 32; ++i) x[i] = 0;
                     }
-                    if (r < count) {
+                    if (staged) {
+                        float v[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = f.wa == 0.f ? 0.f : __uint_as_float(x[i]) * f.wa; // a weight of 0: the sum may be anything
+                        if (f.wb != 0.f) {
+                            float const* base = p.base_out + at * p.d + c * 32;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                if ((uint32_t)(c * 32 + i) < p.d) { // (the head dim is a multiple of 8)
+                                    float4 const b = *reinterpret_cast<float4 const*>(base + i);
+                                    v[i] = fmaf(b.x, f.wb, v[i]);
+                                    v[i + 1] = fmaf(b.y, f.wb, v[i + 1]);
+                                    v[i + 2] = fmaf(b.z, f.wb, v[i + 2]);
+                                    v[i + 3] = fmaf(b.w, f.wb, v[i + 3]);
+                                }
+                            }
+                        }
+                        __syncwarp(); // the chunk before has been read
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) // 16 bytes; four rows share 128 bytes' worth of banks twice
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)),
+                                         "r"(pack_h2(v[8 * i], v[8 * i + 1])), "r"(pack_h2(v[8 * i + 2], v[8 * i + 3])),
+                                         "r"(pack_h2(v[8 * i + 4], v[8 * i + 5])), "r"(pack_h2(v[8 * i + 6], v[8 * i + 7])) : "memory");
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t const rw = (lane >> 2) + 8 * i;
+                            uint4          y;
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                                         : "r"(stage + rw * 64 + (((lane & 3) ^ ((rw >> 1) & 3)) << 4)) : "memory");
+                            if (dst[i] && (uint32_t)(c * 32 + (lane & 3) * 8) < p.d) *reinterpret_cast<uint4*>(dst[i] + c * 32) = y;
+                        }
+                    } else if (r < count) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
                             float const v4[4] = {__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])};
@@ -459,7 +574,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                 split = true;
                 if (threadIdx.x == 0) write_meta<TR>(p, w, true);
             }
-            w = wn;
+            next_item<TR, BK, OVH>(p, w, n);
         }
         if (!split && threadIdx.x == 0) write_meta<TR>(p, w, false);
     }
