@@ -31,8 +31,12 @@ uint64_t align256(uint64_t x)
     return (x + 255) / 256 * 256;
 }
 
+// Partial results of the two kernels that a call may have in flight at once, and a prefix's result
 struct layout_t {
-    uint64_t part_out, part_ml, meta, base_out, base_lse, total;
+    struct region_t {
+        uint64_t out, ml, meta;
+    } region[2];
+    uint64_t base_out, base_lse, total;
 };
 
 layout_t layout(es_paged_attention_t const& a)
@@ -42,25 +46,35 @@ layout_t layout(es_paged_attention_t const& a)
     // of every kernel that the pointers may make the call choose: workers x 2 slots x rows (x head dim)
     uint64_t part = 2ull * SIMT_BLOCKS * 16 * 32, ml = 2ull * SIMT_BLOCKS * 8, meta = SIMT_BLOCKS;
     if (c.dtype == ES_F16 && c.head_dim <= 128) {
-        part = std::max<uint64_t>(part, 2ull * MMA_WORKERS * MMA_MAX_TR * (c.head_dim <= 64 ? 64 : 128));
+        uint64_t const d = c.head_dim <= 64 ? 64 : 128;
+        part = std::max<uint64_t>(part, 2ull * MMA_WORKERS * MMA_MAX_TR * d);
+        part = std::max<uint64_t>(part, 2ull * WIDE_BLOCKS * WIDE_TR * d);
         ml = std::max<uint64_t>(ml, 2ull * MMA_WORKERS * MMA_MAX_TR);
-        meta = std::max<uint64_t>(meta, MMA_WORKERS);
-        part = std::max<uint64_t>(part, 2ull * WIDE_BLOCKS * WIDE_TR * (c.head_dim <= 64 ? 64 : 128));
         ml = std::max<uint64_t>(ml, 2ull * WIDE_BLOCKS * WIDE_TR);
+        meta = std::max<uint64_t>(meta, MMA_WORKERS);
     }
     uint64_t at = 0;
-    l.part_out = at;
-    at += align256(part * 4);
-    l.part_ml = at;
-    at += align256(ml * 8);
-    l.meta = at;
-    at += align256(meta * 2 * 16);
+    for (auto& r : l.region) {
+        r.out = at;
+        at += align256(part * 4);
+        r.ml = at;
+        at += align256(ml * 8);
+        r.meta = at;
+        at += align256(meta * 2 * 16);
+    }
     l.base_out = at;
     if (a.prefix_len) at += align256((uint64_t)c.rows * a.heads * c.head_dim * 4);
     l.base_lse = at;
     if (a.prefix_len) at += align256((uint64_t)c.rows * a.heads * 4);
     l.total = at;
     return l;
+}
+
+void use_region(paged_params_t& p, char* ws, layout_t::region_t const& r)
+{
+    p.part_out = reinterpret_cast<float*>(ws + r.out);
+    p.part_ml = reinterpret_cast<float2*>(ws + r.ml);
+    p.meta = reinterpret_cast<int4*>(ws + r.meta);
 }
 
 unsigned int* error_address()
@@ -86,27 +100,45 @@ bool aligned16(es_paged_attention_t const& a, es_paged_attention_args_t const& x
     return (el % per) == 0 && (bits & 15) == 0 && c.k_stride[1] < (1 << 26) && c.v_stride[1] < (1 << 26);
 }
 
-template <typename T> int launch_simt(paged_params_t& p, bool vec, cudaStream_t stream)
+// One kernel's part of a call: `main` cuts the work into shares, `join` (null: nothing can be split) puts items
+// that crossed shares together.
+struct part_t {
+    paged_params_t p;
+    void (*main)(paged_params_t const&, cudaStream_t);
+    void (*join)(paged_params_t const&, cudaStream_t);
+};
+
+// Tokens an item can have to visit (an upper bound from the descriptor; what there is only the device knows)
+uint64_t most_keys(paged_params_t const& p)
 {
-    uint32_t const nch = p.d <= 64 ? 2 : p.d <= 128 ? 4 : 8;
-    uint32_t const tr = 16 / nch;
-    p.part_d = nch * 32;
+    return p.prefix_len >= 0 ? (uint64_t)p.prefix_len : (uint64_t)p.capacity + p.front;
+}
+
+template <typename T, int NCH, bool VEC> part_t simt_as(paged_params_t p)
+{
+    constexpr uint32_t TR = 16 / NCH;
+    part_t             c;
+    p.part_d = NCH * 32;
     // Direct: with at most 8 key tiles an item, one block an item and no join -- a join costs as much as
     // about 8 tiles take
-    p.direct = !p.row_offsets && p.prefix_len < 0 && p.capacity <= 8 * SIMT_BK;
-    if (p.batch > 65535) p.direct = 0;
-    uint32_t const grid = p.direct ? p.kv_heads * ((p.group + tr - 1) / tr) : SIMT_BLOCKS;
-    auto           go = [&](auto kernel) { launch_k(kernel, dim3(grid, p.direct ? p.batch : 1), dim3(128), 0, stream, p); };
-    if (nch == 2) vec ? go(paged_simt_kernel<T, 2, true>) : go(paged_simt_kernel<T, 2, false>);
-    else if (nch == 4) vec ? go(paged_simt_kernel<T, 4, true>) : go(paged_simt_kernel<T, 4, false>);
-    else vec ? go(paged_simt_kernel<T, 8, true>) : go(paged_simt_kernel<T, 8, false>);
-    if (p.direct) return 1;
-    pdl_scope_t scope(true);
-    auto        join = [&](auto kernel) { launch_k(kernel, dim3(grid), dim3(256), 0, stream, p, vec ? 1 : 0); };
-    if (nch == 2) join(paged_join_kernel<T, 8, 1>);
-    else if (nch == 4) join(paged_join_kernel<T, 4, 1>);
-    else join(paged_join_kernel<T, 2, 2>);
-    return 2;
+    p.direct = !p.row_offsets && p.prefix_len < 0 && most_keys(p) <= 8 * SIMT_BK && p.batch <= 65535;
+    c.p = p;
+    c.main = [](paged_params_t const& p, cudaStream_t s) {
+        dim3 const grid(p.direct ? p.kv_heads * ((p.group + TR - 1) / TR) : SIMT_BLOCKS, p.direct ? p.batch : 1);
+        launch_k(paged_simt_kernel<T, NCH, VEC>, grid, dim3(128), 0, s, p);
+    };
+    c.join = nullptr;
+    if (!p.direct)
+        c.join = [](paged_params_t const& p, cudaStream_t s) {
+            launch_k(paged_join_kernel<T, TR, (NCH * 32 + 127) / 128>, dim3(SIMT_BLOCKS), dim3(256), 0, s, p, VEC ? 1 : 0);
+        };
+    return c;
+}
+template <typename T> part_t simt_part(paged_params_t const& p, bool vec)
+{
+    if (p.d <= 64) return vec ? simt_as<T, 2, true>(p) : simt_as<T, 2, false>(p);
+    if (p.d <= 128) return vec ? simt_as<T, 4, true>(p) : simt_as<T, 4, false>(p);
+    return vec ? simt_as<T, 8, true>(p) : simt_as<T, 8, false>(p);
 }
 
 // Kernels with more shared memory than 48 KB say so once per device
@@ -119,80 +151,94 @@ template <typename K> void allow_smem(K kernel, uint32_t bytes, bool (&done)[64]
     done[dev & 63] = true;
 }
 
-template <int DPAD, int NT, bool PAGE16> void launch_mma_as(paged_params_t const& p, dim3 grid, uint32_t q_rows, cudaStream_t stream)
-{
-    static bool done[64] = {};
-    allow_smem(paged_mma_kernel<DPAD, NT, PAGE16>, MMA_WARPS * mma_warp_bytes<DPAD>(8 * NT), done);
-    launch_k(paged_mma_kernel<DPAD, NT, PAGE16>, grid, dim3(MMA_WARPS * 32), MMA_WARPS * mma_warp_bytes<DPAD>(q_rows), stream, p, q_rows);
-}
-
-template <int NT> int launch_mma(paged_params_t& p, cudaStream_t stream)
+template <int DPAD, int NT, bool PAGE16> part_t mma_as(paged_params_t p)
 {
     constexpr uint32_t TR = 8 * NT;
-    bool const         page16 = p.page.d % MMA_BK == 0;
-    p.part_d = p.d <= 64 ? 64 : 128;
+    part_t             c;
+    p.part_d = DPAD;
     // Direct: with at most 16 key tiles an item, one warp an item and no join
-    p.direct = !p.row_offsets && p.prefix_len < 0 && p.capacity <= 16 * MMA_BK;
+    p.direct = !p.row_offsets && p.prefix_len < 0 && most_keys(p) <= 16 * MMA_BK && p.batch <= 65535;
     p.min_units = 4;
-    if (p.batch > 65535) p.direct = 0;
-    uint32_t const items = p.kv_heads * ((p.group + TR - 1) / TR); // of a sequence
-    dim3 const     grid(p.direct ? (items + MMA_WARPS - 1) / MMA_WARPS : MMA_BLOCKS, p.direct ? p.batch : 1);
-    // rows of a query tile: the packed rows of one token, or of all there are
-    uint32_t const q_rows = std::min<uint32_t>(TR, !p.row_offsets && p.prefix_len < 0 ? p.group : p.rows * p.group);
-    if (p.part_d == 64) page16 ? launch_mma_as<64, NT, true>(p, grid, q_rows, stream) : launch_mma_as<64, NT, false>(p, grid, q_rows, stream);
-    else page16 ? launch_mma_as<128, NT, true>(p, grid, q_rows, stream) : launch_mma_as<128, NT, false>(p, grid, q_rows, stream);
-    if (p.direct) return 1;
-    pdl_scope_t scope(true);
-    launch_k(paged_join_kernel<__half, TR, 1>, dim3(MMA_WORKERS, (TR + 15) / 16), dim3(256), 0, stream, p, 1);
-    return 2;
+    c.p = p;
+    c.main = [](paged_params_t const& p, cudaStream_t s) {
+        static bool done[64] = {};
+        allow_smem(paged_mma_kernel<DPAD, NT, PAGE16>, MMA_WARPS * mma_warp_bytes<DPAD>(TR), done);
+        uint32_t const items = p.kv_heads * ((p.group + TR - 1) / TR); // of a sequence
+        dim3 const     grid(p.direct ? (items + MMA_WARPS - 1) / MMA_WARPS : MMA_BLOCKS, p.direct ? p.batch : 1);
+        // rows of a query tile: the packed rows of one token, or of all there are
+        uint32_t const q_rows = std::min(uint32_t(TR), !p.row_offsets && p.prefix_len < 0 ? p.group : p.rows * p.group);
+        launch_k(paged_mma_kernel<DPAD, NT, PAGE16>, grid, dim3(MMA_WARPS * 32), MMA_WARPS * mma_warp_bytes<DPAD>(q_rows), s, p, q_rows);
+    };
+    c.join = nullptr;
+    if (!p.direct)
+        c.join = [](paged_params_t const& p, cudaStream_t s) {
+            launch_k(paged_join_kernel<__half, TR, 1>, dim3(MMA_WORKERS, (TR + 15) / 16), dim3(256), 0, s, p, 1);
+        };
+    return c;
+}
+template <int NT> part_t mma_part(paged_params_t const& p)
+{
+    bool const page16 = p.page.d % MMA_BK == 0;
+    if (p.d <= 64) return page16 ? mma_as<64, NT, true>(p) : mma_as<64, NT, false>(p);
+    return page16 ? mma_as<128, NT, true>(p) : mma_as<128, NT, false>(p);
 }
 
-template <int DPAD, bool PAGE16> void launch_wide_as(paged_params_t const& p, cudaStream_t stream)
+template <int DPAD, bool PAGE16> part_t wide_as(paged_params_t p)
 {
-    static bool done[64] = {};
-    allow_smem(paged_wide_kernel<DPAD, PAGE16>, wide_smem_bytes<DPAD>(), done);
-    launch_k(paged_wide_kernel<DPAD, PAGE16>, dim3(WIDE_BLOCKS), dim3(WIDE_THREADS), wide_smem_bytes<DPAD>(), stream, p);
-}
-
-int launch_wide(paged_params_t& p, cudaStream_t stream)
-{
-    bool const page16 = p.page.d % 16 == 0;
-    p.part_d = p.d <= 64 ? 64 : 128;
+    part_t c;
+    p.part_d = DPAD;
     p.direct = 0;
     p.min_units = 4;
-    if (p.part_d == 64) page16 ? launch_wide_as<64, true>(p, stream) : launch_wide_as<64, false>(p, stream);
-    else page16 ? launch_wide_as<128, true>(p, stream) : launch_wide_as<128, false>(p, stream);
-    pdl_scope_t scope(true);
-    if (p.part_d == 64) launch_k(paged_wide_join_kernel<64>, dim3(WIDE_BLOCKS, WIDE_TR / 16), dim3(256), 0, stream, p);
-    else launch_k(paged_wide_join_kernel<128>, dim3(WIDE_BLOCKS, WIDE_TR / 16), dim3(256), 0, stream, p);
-    return 2;
+    c.p = p;
+    c.main = [](paged_params_t const& p, cudaStream_t s) {
+        static bool done[64] = {};
+        allow_smem(paged_wide_kernel<DPAD, PAGE16>, wide_smem_bytes<DPAD>(), done);
+        launch_k(paged_wide_kernel<DPAD, PAGE16>, dim3(WIDE_BLOCKS), dim3(WIDE_THREADS), wide_smem_bytes<DPAD>(), s, p);
+    };
+    c.join = [](paged_params_t const& p, cudaStream_t s) {
+        launch_k(paged_wide_join_kernel<DPAD>, dim3(WIDE_BLOCKS, WIDE_TR / 16), dim3(256), 0, s, p);
+    };
+    return c;
+}
+part_t wide_part(paged_params_t const& p)
+{
+    bool const page16 = p.page.d % 16 == 0;
+    if (p.d <= 64) return page16 ? wide_as<64, true>(p) : wide_as<64, false>(p);
+    return page16 ? wide_as<128, true>(p) : wide_as<128, false>(p);
 }
 
-// f16 on the tensor cores: sequences (or the prefix) with up to MMA_MAX_TR packed rows a key head are bound by
-// memory and go to the warp-level units, those with more to tcgen05.  How many rows a sequence has is known on
-// the device when there are row offsets: then both kernels run and each takes its own.
-int launch_phase(paged_params_t& p, int dtype, bool vec, cudaStream_t stream)
+// The kernels of one phase (a prefix, or the sequences' own keys), at most two.  f16 on the tensor cores:
+// sequences (or the prefix) with up to MMA_MAX_TR packed rows a key head are bound by memory and go to the
+// warp-level units, those with more to tcgen05.  How many rows a sequence has is known on the device when there
+// are row offsets: then both kernels run and each takes its own.
+int choose(paged_params_t const& q, int dtype, bool vec, part_t (&c)[2])
 {
+    paged_params_t p = q;
     p.packed_min = 0;
     p.packed_max = 0x7fffffff;
-    if (dtype != ES_F16) return launch_simt<float>(p, vec, stream);
-    if (!vec || p.d > 128) return launch_simt<__half>(p, vec, stream);
+    if (dtype != ES_F16) {
+        c[0] = simt_part<float>(p, vec);
+        return 1;
+    }
+    if (!vec || p.d > 128) {
+        c[0] = simt_part<__half>(p, vec);
+        return 1;
+    }
     // packed rows of an item: one token's, those of all rows there are, or (row offsets) something in between
     uint32_t const most = p.prefix_len < 0 && !p.row_offsets ? p.group : p.rows * p.group;
     uint32_t const fewest = p.row_offsets ? 1 : most;
-    int            launches = 0;
+    int            n = 0;
     if (fewest <= MMA_MAX_TR) {
         p.packed_max = MMA_MAX_TR;
         uint32_t const rows = p.prefix_len >= 0 ? most : p.group; // of an item, where tokens come singly
-        launches += rows <= 8 ? launch_mma<1>(p, stream) : rows <= 16 ? launch_mma<2>(p, stream) : launch_mma<4>(p, stream);
+        c[n++] = rows <= 8 ? mma_part<1>(p) : rows <= 16 ? mma_part<2>(p) : mma_part<4>(p);
     }
     if (most > MMA_MAX_TR) {
-        pdl_scope_t scope(launches > 0 || pdl_launch_flag());
         p.packed_min = MMA_MAX_TR;
         p.packed_max = 0x7fffffff;
-        launches += launch_wide(p, stream);
+        c[n++] = wide_part(p);
     }
-    return launches;
+    return n;
 }
 
 } // namespace
@@ -245,9 +291,6 @@ int launch_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
     p.row_offsets = x.row_offsets;
     p.lengths = x.lengths;
     p.tables = x.tables;
-    p.part_out = reinterpret_cast<float*>(ws + l.part_out);
-    p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
-    p.meta = reinterpret_cast<int4*>(ws + l.meta);
     for (int i = 0; i != 2; ++i) {
         p.q_stride[i] = a.q_stride[i];
         p.out_stride[i] = a.out_stride[i];
@@ -273,8 +316,19 @@ int launch_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
     p.scale_log2 = a.scale * LOG2_E;
     p.error = error_address();
     bool const vec = aligned16(a, x);
-    int        launches = 0;
-    if (a.prefix_len) {
+    // A short prefix is read by every sequence for itself, in front of its own keys and out of the L2 cache:
+    // with up to 64 MB read in all that takes less than the two kernels that reading it once would add (3
+    // sequences behind 500 tokens: 25 us shared, 11 us so).  Single tokens only: parts of prompts have rows
+    // enough to share.
+    uint64_t const all = (uint64_t)c.batch * a.prefix_len * c.kv_heads * c.head_dim * 2 * dtype_size(c.dtype);
+    bool const     front = a.prefix_len && !x.row_offsets && p.group <= MMA_MAX_TR && all <= (64ull << 20);
+    int            launches = 0;
+    bool const     pdl = pdl_launch_flag();
+    auto           next = [&] { return pdl_scope_t(launches++ > 0 || pdl); };
+    if (front) {
+        p.front = a.prefix_len;
+        p.front_pages = x.prefix_pages;
+    } else if (a.prefix_len) {
         paged_params_t f = p;
         f.prefix_len = (int32_t)a.prefix_len;
         f.tables = x.prefix_pages;
@@ -282,12 +336,43 @@ int launch_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
         f.out = ws + l.base_out;
         f.out_f32 = 1;
         f.lse = reinterpret_cast<float*>(ws + l.base_lse);
-        launches += launch_phase(f, c.dtype, vec, stream);
+        part_t    k[2];
+        int const n = choose(f, c.dtype, vec, k);
+        for (int i = 0; i != n; ++i) {
+            use_region(k[i].p, ws, l.region[0]);
+            k[i].p.order = i == 0 && n == 1 ? ORDER_FIRST : ORDER_PLAIN;
+            {
+                auto scope = next();
+                k[i].main(k[i].p, stream);
+            }
+            if (k[i].join) {
+                auto scope = next();
+                k[i].join(k[i].p, stream);
+            }
+        }
+        // the sequences' own keys need the prefix's result only where a row is finished
+        p.order = n == 1 ? ORDER_LATE : ORDER_PLAIN;
         p.base_out = reinterpret_cast<float const*>(ws + l.base_out);
         p.base_lse = reinterpret_cast<float const*>(ws + l.base_lse);
     }
-    pdl_scope_t scope(launches > 0 || pdl_launch_flag());
-    launches += launch_phase(p, c.dtype, vec, stream);
+    part_t    k[2];
+    int const n = choose(p, c.dtype, vec, k);
+    if (n == 2 && p.order == ORDER_PLAIN) { // independent of one another
+        k[0].p.order = ORDER_FIRST;
+        k[1].p.order = ORDER_LATE;
+    } else if (n == 2) {
+        k[0].p.order = k[1].p.order = ORDER_PLAIN;
+    }
+    for (int i = 0; i != n; ++i) {
+        use_region(k[i].p, ws, l.region[n == 2 ? i : 1]);
+        auto scope = next();
+        k[i].main(k[i].p, stream);
+    }
+    for (int i = 0; i != n; ++i) {
+        if (!k[i].join) continue;
+        auto scope = next();
+        k[i].join(k[i].p, stream);
+    }
     return launches;
 }
 

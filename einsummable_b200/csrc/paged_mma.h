@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(i), "r"(0) : "memory");
         __syncwarp();
     }
-    ES_PDL_PROLOGUE();
+    begin_order(p);
     work_t w;
     find_work<TR, BK, OVH, THREADS, MMA_WARPS>(p, w, sched);
     bool split = false;
@@ -108,6 +108,9 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
         bool           first_tile = true; // of an item
         __half const  *ks = nullptr, *vs = nullptr; // this lane's part of the next tile's first rows
         uint32_t       slot = 0, page_no = 0, page_next = 0;
+        uint32_t const fronts = (p.front + BK - 1) / BK; // key tiles in front of a sequence's own
+        int32_t const* table = nullptr;                  // the pages being read and the tokens in them
+        int            len = 0;
         // next tile of the item in a new page: its number was fetched a page ahead
         auto enter_page = [&](uint32_t page) {
             if (page >= p.n_pages) { // reported where it was found; reads page 0, which is there
@@ -119,11 +122,17 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
             vs = static_cast<__half const*>(p.v) + (int64_t)page * p.v_stride[0] + (int64_t)(slot + c_row) * p.v_stride[1] +
                  (int64_t)wl.head * p.v_stride[2] + c_chunk * 8;
             ++page_no;
-            if ((uint64_t)page_no * p.page.d < (uint32_t)wl.s.len) page_next = (uint32_t)wl.s.table[page_no];
+            if ((uint64_t)page_no * p.page.d < (uint32_t)len) page_next = (uint32_t)table[page_no];
         };
         auto issue = [&]() { // one tile's copies (or none) and their group
             if (wl.left && to_next_tile<OVH>(wl)) {
-                int const key0 = (int)((wl.j - OVH) * BK);
+                uint32_t const tile = wl.j - OVH;
+                bool const     front = tile < fronts, enter = first_tile || tile == fronts;
+                int const      key0 = (int)((front ? tile : tile - fronts) * BK);
+                if (enter) {
+                    table = front ? p.front_pages : wl.s.table;
+                    len = front ? (int)p.front : wl.s.len;
+                }
                 if (first_tile) {
                     first_tile = false;
                     uint32_t const start = wl.t * TR;
@@ -134,13 +143,13 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                                             (int64_t)(wl.head * p.group + (pr - tok * p.group)) * p.q_stride[1] + c_chunk * 8;
                         if (c_on) copy16(fill + 2 * TILE + r * ROW + ((c_chunk ^ (r & 7)) << 4), src, true);
                     }
-                    if (PAGE16 && key0 < wl.s.len) {
-                        page_no = fdivide((uint32_t)key0, p.page);
-                        slot = (uint32_t)key0 - page_no * p.page.d;
-                        enter_page((uint32_t)wl.s.table[page_no]);
-                    }
                 }
-                if (PAGE16 && key0 + BK <= wl.s.len) {
+                if (PAGE16 && enter && key0 < len) {
+                    page_no = fdivide((uint32_t)key0, p.page);
+                    slot = (uint32_t)key0 - page_no * p.page.d;
+                    enter_page((uint32_t)table[page_no]);
+                }
+                if (PAGE16 && key0 + BK <= len) {
                     if (slot == p.page.d) {
                         slot = 0;
                         enter_page(page_next);
@@ -159,9 +168,9 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                     // the sequence's last, incomplete tile, or pages that end inside tiles: lane r < 16 finds key r
                     int64_t ko = 0, vo = 0;
                     bool    ok = false;
-                    if (lane < BK && key0 + lane < wl.s.len) {
+                    if (lane < BK && key0 + lane < len) {
                         uint32_t const key = (uint32_t)(key0 + lane), pi = fdivide(key, p.page);
-                        uint32_t const page = (uint32_t)wl.s.table[pi], at = key - pi * p.page.d;
+                        uint32_t const page = (uint32_t)table[pi], at = key - pi * p.page.d;
                         ok = page < p.n_pages;
                         if (!ok) report(p, PAGED_BAD_PAGE);
                         ko = (int64_t)page * p.k_stride[0] + (int64_t)at * p.k_stride[1] + (int64_t)wl.head * p.k_stride[2];
@@ -223,7 +232,9 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
             }
             int const vis_all = visible(p, w.s, (int)fdivide(start, p.grp)); // keys that every row of the tile sees
             uint32_t const n_tiles = first_tile_of<OVH>(w.j + n_units) - first_tile_of<OVH>(w.j);
-            int            key0 = (int)(first_tile_of<OVH>(w.j) * BK);
+            // number of the tile's first key among the sequence's own; of a key in front: negative
+            int const fronts = (int)((p.front + BK - 1) / BK * BK);
+            int       key0 = (int)(first_tile_of<OVH>(w.j) * BK) - fronts;
 #pragma unroll 1
             for (uint32_t u = 0; u < n_tiles; ++u) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(MMA_STAGES - 2) : "memory");
@@ -259,12 +270,13 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[nt][0][i] += s[nt][1][i];
-                if (key0 + BK > vis_all) {
+                int const limit = (int)p.front - fronts; // keys in front end here
+                if (key0 < 0 ? key0 + BK > limit : key0 + BK > vis_all) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (key0 + g + 8 * (i >> 1) >= vis[nt][i & 1]) s[nt][0][i] = -INFINITY; // (the scale is positive)
+                            if (key0 + g + 8 * (i >> 1) >= (key0 < 0 ? limit : vis[nt][i & 1])) s[nt][0][i] = -INFINITY; // (the scale is positive)
                 }
                 key0 += BK;
                 bool over = false; // a score beyond the running maximum
@@ -318,6 +330,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                 st = st + stage_bytes == ring_end ? ring : st + stage_bytes;
             }
             int const to = segment_slot(w, n_units);
+            if (to < 0 && p.base_out) wait_for_base(p);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -388,6 +401,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
         asm volatile("cp.async.wait_all;" ::: "memory");
     }
     if (!split && !p.direct && lane == 0) write_meta<TR>(p, w, false);
+    wait_for_base(p);
 }
 
 } // namespace

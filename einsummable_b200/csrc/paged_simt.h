@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
     __shared__ sched_smem_t<NT, 1> sched;
     __shared__ float            so[4][TR][NCH * 32];
     __shared__ float2           sml[4][TR];
-    ES_PDL_PROLOGUE();
+    begin_order(p);
     int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, stream = threadIdx.x >> 3;
     work_t    w;
     find_work<TR, BK, OVH, NT, 1>(p, w, sched);
@@ -71,14 +71,18 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
                 for (int i = 0; i < 4; ++i) q[r][c][i] *= p.scale_log2;
             }
         }
+        // keys are numbered from the first of those in front on, the sequence's own from `own` on
+        int const own = (int)((p.front + BK - 1) / BK * BK);
         int const key_begin = (int)(first_tile_of<OVH>(w.j) * BK);
-        int const key_end = (int)min((uint64_t)first_tile_of<OVH>(w.j + n_units) * BK, (uint64_t)vis_max);
+        int const key_end = (int)min((uint64_t)first_tile_of<OVH>(w.j + n_units) * BK, (uint64_t)own + (uint64_t)vis_max);
         T const*  kb = static_cast<T const*>(p.k) + (int64_t)w.head * p.k_stride[2];
         T const*  vb = static_cast<T const*>(p.v) + (int64_t)w.head * p.v_stride[2];
         auto      load = [&](int key, float (&k)[NCH][4], float (&v)[NCH][4]) -> bool {
-            if (key >= key_end) return false;
+            if (key >= key_end || (key < own && key >= (int)p.front)) return false;
+            int32_t const* table = key < own ? p.front_pages : w.s.table;
+            if (key >= own) key -= own;
             uint32_t const pi = fdivide((uint32_t)key, p.page);
-            uint32_t const page = (uint32_t)w.s.table[pi];
+            uint32_t const page = (uint32_t)table[pi];
             if (page >= p.n_pages) {
                 report(p, PAGED_BAD_PAGE);
                 return false;
@@ -117,7 +121,7 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
                 s += __shfl_xor_sync(0xffffffffu, s, 4);
                 s += __shfl_xor_sync(0xffffffffu, s, 2);
                 s += __shfl_xor_sync(0xffffffffu, s, 1);
-                if (have && key < vis[r]) {
+                if (have && key - own < vis[r]) {
                     if (s > m[r]) {
                         float const a = ex2(m[r] - s); // m = -inf: 0
                         m[r] = s;
@@ -172,6 +176,7 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
         }
         __syncthreads();
         int const slot = segment_slot(w, n_units);
+        if (slot < 0 && p.base_out) wait_for_base(p);
         // the four warps' results; a thread 4 elements of a row
         for (int x = threadIdx.x; x < count * NCH * 8; x += NT) {
             int const      r = x / (NCH * 8);
@@ -215,6 +220,7 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
         next_item<TR, BK, OVH>(p, w, n_units);
     }
     if (!split && !p.direct && threadIdx.x == 0) write_meta<TR>(p, w, false);
+    wait_for_base(p);
 }
 
 } // namespace

@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     uint32_t const tmem = ctrl->tmem_base; // scores: + 128 t; accumulators: + 256 + 128 t
-    ES_PDL_PROLOGUE();
+    begin_order(p);
     work_t w;
     find_work<TR, BK, OVH, WIDE_THREADS, 1>(p, w, sched);
 
@@ -492,6 +492,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                 uint32_t const head = w.head * p.group + (pr - tok * p.group);
                 uint64_t const at = (uint64_t)row * p.heads + head, part = (uint64_t)(2 * w.worker + max(to, 0)) * TR + r;
                 finish_t       f = {0.f, 0.f, 0.f};
+                if (to < 0 && p.base_out) wait_for_base(p);
                 if (to < 0 && r < count) {
                     f = finish(m, l, p.base_lse != nullptr, p.base_lse ? p.base_lse[at] : 0.f);
                     if (p.lse) p.lse[at] = f.lse;
@@ -578,6 +579,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
         }
         if (!split && threadIdx.x == 0) write_meta<TR>(p, w, false);
     }
+    wait_for_base(p);
     // ------------------------------------------------------------------ teardown
     tc_fence_before();
     __syncthreads();

@@ -44,13 +44,34 @@ struct paged_params_t {
     fastdiv_t      page, grp;
     int32_t        causal;
     int32_t        prefix_len;  // >= 0: all rows attend the one list of pages `tables`, of this many tokens
+    int32_t const* front_pages; // front > 0: so many tokens, listed here, lie in front of every sequence's own (each
+    uint32_t       front;       // sequence reads them for itself); their last key tile is not shared with its own
     int32_t        direct;      // one worker an item: nothing is split (one row a sequence)
     uint32_t       packed_min, packed_max; // sequences with more than / at most so many packed rows
     uint32_t       min_units;   // a worker's share is at least this
     float          scale_log2;  // scale * log2 e
     int32_t        out_f32;
+    int32_t        order;       // ORDER_*: when the kernel waits for the kernels before it
     unsigned int*  error;
 };
+
+// Programmatic dependent launch between the kernels of one call (pdl.h).  A kernel starts when the one before it
+// has let it; what it may touch then is another matter:
+//   ORDER_PLAIN  lets the next one start at once and waits for the kernels before it
+//   ORDER_FIRST  waits, then lets the next one start: whoever starts after it finds the call's inputs ready
+//   ORDER_LATE   needs nothing of the kernel before it but a prefix's result, if that: it waits before it reads
+//                that, and before it ends (the kernel behind it waits for this one alone)
+enum { ORDER_PLAIN = 0, ORDER_FIRST = 1, ORDER_LATE = 2 };
+__device__ __forceinline__ void begin_order(paged_params_t const& p)
+{
+    if (p.order != ORDER_FIRST) asm volatile("griddepcontrol.launch_dependents;");
+    if (p.order != ORDER_LATE) ES_PDL_WAIT();
+    if (p.order == ORDER_FIRST) asm volatile("griddepcontrol.launch_dependents;");
+}
+__device__ __forceinline__ void wait_for_base(paged_params_t const& p)
+{
+    if (p.order == ORDER_LATE) ES_PDL_WAIT();
+}
 
 __device__ __forceinline__ void report(paged_params_t const& p, unsigned code)
 {
@@ -114,7 +135,7 @@ template <int TR, int BK, int OVH> __device__ __forceinline__ uint32_t tile_unit
 {
     uint32_t const last = min((t + 1) * TR, (uint32_t)s.n * p.group) - 1;
     uint32_t const keys = (uint32_t)visible(p, s, (int)fdivide(last, p.grp));
-    return max(1u, (keys + BK - 1) / BK) + OVH;
+    return max(1u, (keys + BK - 1) / BK + (p.front + BK - 1) / BK) + OVH;
 }
 template <int TR> __device__ __forceinline__ uint32_t row_tiles(paged_params_t const& p, sequence_t const& s)
 {

@@ -104,6 +104,13 @@ PREFIX = [
     ([1] * 6, [3, 0, 17, 90, 300, 2], 8, 4, 64, 16, 333, {"dtype": "f32"}),
     ([1] * 6, [3, 0, 17, 90, 300, 2], 8, 4, 100, 16, 333, {"layout": "odd"}),
     ([1] * 130, [i % 5 for i in range(130)], 2, 1, 128, 64, 4000, {}),
+    # the prefix read once for few rows, on the tensor cores and without
+    ([1] * 3, [0, 31, -1], 32, 8, 128, 16, 6000, {}),
+    ([1] * 4, [5, 0, 70, -1], 8, 4, 64, 16, 500, {"offsets": True}),
+    ([1] * 4, [5, 0, 70, -1], 8, 4, 64, 16, 500, {"offsets": True, "dtype": "f32"}),
+    ([1] * 4, [5, 0, 70, 260], 8, 4, 64, 16, 15, {}),               # a prefix that ends inside a key tile
+    ([1] * 9, [5, 0, 70, 260, 1, 2, 3, 4, 5], 8, 4, 64, 24, 100, {}),
+    ([1] * 40, [i for i in range(40)], 32, 1, 128, 16, 200, {"offsets": True}),  # 32 heads on one key head: 1280 rows
 ]
 
 
