@@ -3,12 +3,13 @@
 //   p = L_i - n_i + r,   (x, y)_j <- (x cos - y sin, x sin + y cos)_j with angle table entry f[p + offset, j]
 //   K[table_i[p / page], p % page] <- rotated k_r,   V[...] <- v_r,   q_out_r <- rotated q_r
 //
-// Bound: memory (each element is read and written once; 3 flops an element).  One thread moves 8
-// elements of a head (16 bytes of f16), or 2 + 2 runs of 4 that belong together when a pair's members are
-// half a head apart; neighbouring threads on neighbouring elements.  A block takes a token's whole row of
-// heads at a time, so that the token's sequence, page and angles are found once a block: the sequence by
-// counting, with all threads at once, how many sequences end at or before the row (one round of loads, not a
-// chain of log2(batch) dependent ones).
+// Bound: memory (each element is read and written once; 3 flops an element), and close behind it the number of
+// instructions a move takes.  A thread moves 8 elements of a head -- 16 bytes of f16, or 2 runs of 4 when a pair's
+// members are half a head apart.  A block moves one of the three tensors, so that nothing about a move is decided by
+// thread, for several rows: what a row needs to know first is a chain of loads -- its sequence (found by counting, a
+// lane a sequence, how many end at or before the row), the sequence's length, the page -- and a block's warps find
+// the places of all its rows before it moves them.  Moves are short chains of loads, so warps count: 40 an SM.  The
+// blocks make one wave.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -39,8 +40,8 @@ struct append_params_t {
     int64_t        pos_offset;
     uint64_t       n_positions;
     uint32_t       batch, rows, heads, kv_heads, d, rot, n_pages, table_stride, capacity;
-    uint32_t       units_per_head; // threads a head
-    fastdiv_t      page, upd; // page_size; units per head
+    fastdiv_t      page, upd, by_heads[2]; // page_size; units a head; heads of the queries, of keys and values
+    uint32_t       first_block[2], rows_a_block[2];
 };
 
 template <typename T, int N> struct vec_t;
@@ -90,136 +91,183 @@ template <int N, bool VEC, typename T> __device__ __forceinline__ void store_n(T
     }
 }
 
-// One unit of a head: adjacent pairs: 8 elements from 8u on.  Halves: unit u of the first rot / 8 ones holds
-// elements 4u.. and rot/2 + 4u.., the units behind them 8 elements each from `rot` on.
-template <typename TI, typename TC, bool HALVES, bool VEC>
-__device__ __forceinline__ void move_unit(TI const* src, TC* dst, uint32_t u, uint32_t d, uint32_t rot, float const* f)
+// The 8 elements of unit u of a head.  Adjacent pairs: from 8u on.  Halves: unit u of the first ceil(rot / 8)
+// holds 4u.. and rot / 2 + 4u.., the units behind them 8 elements each from `rot` on.
+struct unit_t {
+    uint32_t e0, e1; // where its two runs of 4 begin (one run of 8: e1 = e0 + 4)
+    int      n0, n1; // elements of each that exist
+    bool     rotated;
+};
+template <bool HALVES> __device__ __forceinline__ unit_t unit_of(uint32_t u, uint32_t d, uint32_t rot)
 {
-    if constexpr (HALVES) {
-        uint32_t const half = rot / 2, n_rot = (half + 3) / 4;
-        if (u < n_rot) {
-            uint32_t const e = 4 * u;
-            int const      n = min(4, (int)(half - e));
-            float          a[4], b[4], c[8];
-            load_n<4, VEC>(src + e, a, n);
-            load_n<4, VEC>(src + half + e, b, n);
-            load_n<8, VEC>(f + 2 * e, c, 2 * n);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float const x = a[j], y = b[j];
-                a[j] = x * c[2 * j] - y * c[2 * j + 1];
-                b[j] = x * c[2 * j + 1] + y * c[2 * j];
-            }
-            store_n<4, VEC>(dst + e, a, n);
-            store_n<4, VEC>(dst + half + e, b, n);
-        } else {
-            uint32_t const e = rot + 8 * (u - n_rot);
-            int const      n = min(8, (int)(d - e));
-            float          x[8];
-            load_n<8, VEC>(src + e, x, n);
-            store_n<8, VEC>(dst + e, x, n);
-        }
+    unit_t         t;
+    uint32_t const half = rot / 2, n_rot = (half + 3) / 4;
+    if (HALVES && u < n_rot) {
+        t.e0 = 4 * u;
+        t.e1 = half + 4 * u;
+        t.n0 = t.n1 = min(4, (int)(half - t.e0));
+        t.rotated = true;
     } else {
-        uint32_t const e = 8 * u;
-        int const      n = min(8, (int)(d - e));
-        float          x[8], c[8];
-        load_n<8, VEC>(src + e, x, n);
-        if (e < rot) {
-            int const nr = min(n, (int)(rot - e)); // even
-            if (VEC && nr == 8) {
-                load_n<8, true>(f + e, c, 8);
-            } else {
-                load_n<8, false>(f + e, c, nr);
-            }
+        t.e0 = HALVES ? rot + 8 * (u - n_rot) : 8 * u;
+        t.e1 = t.e0 + 4;
+        t.n0 = min(4, (int)d - (int)t.e0);
+        t.n1 = min(4, (int)d - (int)t.e1);
+        t.rotated = !HALVES && t.e0 < rot;
+    }
+    return t;
+}
+
+// (as they lie in memory: converted when their turn comes)
+template <typename T> struct alignas(16) raw_t {
+    T v[8];
+};
+template <bool HALVES, bool VEC, typename T> __device__ __forceinline__ void load_unit(T const* p, unit_t const& t, raw_t<T>& x)
+{
+    if constexpr (VEC && !HALVES) {
+        x = *reinterpret_cast<raw_t<T> const*>(p + t.e0);
+    } else if constexpr (VEC) {
+        *reinterpret_cast<vec_t<T, 4>*>(&x.v[0]) = *reinterpret_cast<vec_t<T, 4> const*>(p + t.e0);
+        *reinterpret_cast<vec_t<T, 4>*>(&x.v[4]) = *reinterpret_cast<vec_t<T, 4> const*>(p + t.e1);
+    } else {
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                if (j < nr) {
-                    float const a = x[j], b = x[j + 1];
-                    x[j] = a * c[j] - b * c[j + 1];
-                    x[j + 1] = a * c[j + 1] + b * c[j];
-                }
-            }
+        for (int j = 0; j < 4; ++j) {
+            if (j < t.n0) x.v[j] = p[t.e0 + j];
+            if (j < t.n1) x.v[4 + j] = p[t.e1 + j];
         }
-        store_n<8, VEC>(dst + e, x, n);
+    }
+}
+template <bool HALVES, bool VEC, typename T> __device__ __forceinline__ void store_unit(T* p, unit_t const& t, float const (&x)[8])
+{
+    if constexpr (VEC && !HALVES) {
+        store_n<8, true>(p + t.e0, x, 8);
+    } else {
+        float const a[4] = {x[0], x[1], x[2], x[3]}, b[4] = {x[4], x[5], x[6], x[7]};
+        store_n<4, VEC>(p + t.e0, a, t.n0);
+        store_n<4, VEC>(p + t.e1, b, t.n1);
+    }
+}
+// c: cosine and sine of the unit's four pairs
+template <bool HALVES> __device__ __forceinline__ void rotate(float (&x)[8], float const (&c)[8])
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        int const   i0 = HALVES ? j : 2 * j, i1 = HALVES ? 4 + j : 2 * j + 1;
+        float const a = x[i0], b = x[i1];
+        x[i0] = a * c[2 * j] - b * c[2 * j + 1];
+        x[i1] = a * c[2 * j + 1] + b * c[2 * j];
     }
 }
 
-template <typename TI, typename TC, bool HALVES, bool VEC>
-__global__ void __launch_bounds__(256) cache_append_kernel(const __grid_constant__ append_params_t p)
+constexpr uint32_t ROWS_MAX = 64, APPEND_THREADS = 256;
+constexpr uint32_t blocks_an_sm(bool f16_rows) { return f16_rows ? 5 : 3; } // (what their registers leave room for)
+
+struct place_t { // of a row, in one tensor
+    int64_t to;    // element of the tensor written to, without the head; < 0: the row is not moved
+    int64_t angle; // element of the table of angles
+};
+
+// (what: 0 queries, 1 keys, 2 values; all lanes of a warp call)
+__device__ __forceinline__ place_t find_place(append_params_t const& p, uint32_t row, int what)
 {
+    place_t   t = {-1, 0};
+    int const lane = threadIdx.x & 31;
+    auto      report = [&](unsigned code) {
+        if (lane == 0) atomicCAS(&g_append_error, 0u, code);
+        return t;
+    };
+    int seq = (int)row, back = 1; // rows from this one to the end of its sequence
+    if (p.row_offsets) {
+        seq = 0; // sequences that end at or before this row
+        for (uint32_t i0 = 0; i0 < p.batch; i0 += 32)
+            seq += __popc(__ballot_sync(0xffffffffu, i0 + lane < p.batch && p.row_offsets[i0 + lane + 1] <= (int)row));
+        if (seq >= (int)p.batch) return t; // padding
+        int const a = p.row_offsets[seq], b = p.row_offsets[seq + 1];
+        back = b - (int)row;
+        if (a < 0 || a > (int)row || back <= 0 || b > (int)p.rows) return report(PAGED_BAD_ROWS); // offsets that fall, or pass the rows
+    }
+    int const length = p.lengths[seq];
+    if (length < 0 || (uint32_t)length > p.capacity) return report(PAGED_BAD_LENGTH);
+    int const pos = length - back;
+    if (pos < 0) return t; // no place in the cache
+    uint64_t const angle = (uint64_t)(pos + p.pos_offset);
+    if (p.rot && angle >= p.n_positions) return report(PAGED_BAD_POSITION);
+    t.angle = (int64_t)(angle * p.rot);
+    if (what == 0) {
+        t.to = (int64_t)row * p.q_out_stride[0];
+        return t;
+    }
+    uint32_t const pi = fdivide((uint32_t)pos, p.page);
+    uint32_t const slot = (uint32_t)pos - pi * p.page.d;
+    uint32_t const page = (uint32_t)p.tables[(uint64_t)seq * p.table_stride + pi];
+    if (page >= p.n_pages) return report(PAGED_BAD_PAGE);
+    int64_t const* so = what == 1 ? p.kc_stride : p.vc_stride;
+    t.to = (int64_t)page * so[0] + (int64_t)slot * so[1];
+    return t;
+}
+
+// Blocks [0, first_block[0]) move queries, [.., first_block[1]) keys, the others values, rows_a_block[.] rows each.
+// A thread keeps its unit and steps through heads and rows by adding strides.
+template <typename TI, typename TC, bool HALVES, bool VEC>
+__global__ void __launch_bounds__(APPEND_THREADS, blocks_an_sm(sizeof(TI) == 2 && VEC)) cache_append_kernel(const __grid_constant__ append_params_t p)
+{
+    __shared__ place_t places[ROWS_MAX];
     ES_PDL_PROLOGUE();
-    uint32_t const n_heads = p.heads + 2 * p.kv_heads;
-    uint32_t const units = n_heads * p.units_per_head;
-    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        // the row's sequence and position
-        int  seq = (int)row;
-        int  back = 1; // rows from this one to the end of its sequence
-        bool used = true;
-        if (p.row_offsets) {
-            int below = 0; // sequences that end at or before this row
-            for (uint32_t i0 = 0; i0 < p.batch; i0 += blockDim.x) {
-                uint32_t const i = i0 + threadIdx.x;
-                below += __syncthreads_count(i < p.batch && p.row_offsets[i + 1] <= (int)row);
-            }
-            seq = below;
-            used = seq < (int)p.batch;
-            if (used) {
-                int const a = p.row_offsets[seq], b = p.row_offsets[seq + 1];
-                back = b - (int)row;
-                if (a < 0 || a > (int)row || back <= 0 || b > (int)p.rows) { // offsets that fall, or pass the rows
-                    if (threadIdx.x == 0) atomicCAS(&g_append_error, 0u, (unsigned)PAGED_BAD_ROWS);
-                    used = false;
-                }
+    int const      what = blockIdx.x < p.first_block[0] ? 0 : blockIdx.x < p.first_block[1] ? 1 : 2;
+    uint32_t const block = blockIdx.x - (what ? p.first_block[what - 1] : 0), per = p.rows_a_block[what != 0];
+    uint32_t const row0 = block * per, rows = min(per, p.rows - row0);
+    for (uint32_t r = threadIdx.x >> 5; r < rows; r += APPEND_THREADS / 32) {
+        place_t const w = find_place(p, row0 + r, what);
+        if ((threadIdx.x & 31) == 0) places[r] = w;
+    }
+    uint32_t const heads = what ? p.kv_heads : p.heads;
+    uint32_t const at_once = APPEND_THREADS / p.upd.d; // heads that the block moves at once: of one row, or of several rows
+    uint32_t const mine = fdivide(threadIdx.x, p.upd), u = threadIdx.x - mine * p.upd.d;
+    uint32_t const rows_at_once = max(at_once / heads, 1u), row_off = heads < at_once ? fdivide(mine, p.by_heads[what != 0]) : 0;
+    uint32_t const h0 = mine - row_off * heads;
+    bool const     on = mine < at_once && row_off < rows_at_once && h0 < heads;
+    unit_t const   t = unit_of<HALVES>(u, p.d, p.rot);
+    bool const     turn = what != 2 && t.rotated;
+    int64_t const  si0 = (what == 0 ? p.q_stride : what == 1 ? p.k_stride : p.v_stride)[0];
+    int64_t const  si1 = (what == 0 ? p.q_stride : what == 1 ? p.k_stride : p.v_stride)[1];
+    int64_t const  so1 = what == 0 ? p.q_out_stride[1] : what == 1 ? p.kc_stride[2] : p.vc_stride[2];
+    TI const*      src = static_cast<TI const*>(what == 0 ? p.q : what == 1 ? p.k : p.v) + (int64_t)(row0 + row_off) * si0 + (int64_t)h0 * si1;
+    TC*            dst = static_cast<TC*>(what == 0 ? p.q_out : what == 1 ? p.k_cache : p.v_cache) + (int64_t)h0 * so1;
+    float const*   angles = p.freqs + (HALVES ? 2 * t.e0 : t.e0); // rot / 2 pairs of floats a position
+    __syncthreads();
+    if (!on) return;
+    for (uint32_t r = row_off; r < rows; r += rows_at_once, src += rows_at_once * si0) {
+        place_t const at = places[r];
+        if (at.to < 0) continue;
+        float c[8];
+        if (turn) {
+            float const* f = angles + at.angle;
+            if (VEC) {
+                load_n<8, true>(f, c, 8);
+            } else {
+                int const n = HALVES ? 2 * t.n0 : min(8, (int)(p.rot - t.e0));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) c[j] = j < n ? f[j] : (j & 1 ? 0.f : 1.f); // pairs that are not rotated stay what they are
             }
         }
-        if (!used) continue; // (uniform in the block, as is every branch up to the units)
-        int const length = p.lengths[seq];
-        if (length < 0 || (uint32_t)length > p.capacity) {
-            if (threadIdx.x == 0) atomicCAS(&g_append_error, 0u, (unsigned)PAGED_BAD_LENGTH);
-            continue;
-        }
-        int const pos = length - back;
-        if (pos < 0) continue; // no place in the cache
-        uint32_t const pi = fdivide((uint32_t)pos, p.page);
-        uint32_t const slot = (uint32_t)pos - pi * p.page.d;
-        uint32_t const page = (uint32_t)p.tables[(uint64_t)seq * p.table_stride + pi];
-        uint64_t const angle = (uint64_t)(pos + p.pos_offset);
-        bool const     page_ok = page < p.n_pages, angle_ok = p.rot == 0 || angle < p.n_positions;
-        if (threadIdx.x == 0 && !page_ok) atomicCAS(&g_append_error, 0u, (unsigned)PAGED_BAD_PAGE);
-        if (threadIdx.x == 0 && !angle_ok) atomicCAS(&g_append_error, 0u, (unsigned)PAGED_BAD_POSITION);
-        if (!angle_ok) continue;
-        float const* f = p.freqs + angle * p.rot; // rot / 2 pairs of floats
-        TC* const    kc = static_cast<TC*>(p.k_cache) + (int64_t)page * p.kc_stride[0] + (int64_t)slot * p.kc_stride[1];
-        TC* const    vc = static_cast<TC*>(p.v_cache) + (int64_t)page * p.vc_stride[0] + (int64_t)slot * p.vc_stride[1];
-        // blockIdx.y shares out a row's units when there are few rows
-        for (uint32_t w = blockIdx.y * blockDim.x + threadIdx.x; w < units; w += gridDim.y * blockDim.x) {
-            uint32_t const head = fdivide(w, p.upd);
-            uint32_t const u = w - head * p.units_per_head;
-            if (head < p.heads) {
-                move_unit<TI, TC, HALVES, VEC>(
-                    static_cast<TI const*>(p.q) + (int64_t)row * p.q_stride[0] + (int64_t)head * p.q_stride[1],
-                    static_cast<TC*>(p.q_out) + (int64_t)row * p.q_out_stride[0] + (int64_t)head * p.q_out_stride[1], u, p.d,
-                    p.rot, f);
-            } else if (page_ok) {
-                uint32_t const hk = head - p.heads;
-                if (hk < p.kv_heads) {
-                    move_unit<TI, TC, HALVES, VEC>(
-                        static_cast<TI const*>(p.k) + (int64_t)row * p.k_stride[0] + (int64_t)hk * p.k_stride[1],
-                        kc + (int64_t)hk * p.kc_stride[2], u, p.d, p.rot, f);
-                } else {
-                    uint32_t const hv = hk - p.kv_heads;
-                    // values are not rotated: with halves the unit's two runs are moved as they are
-                    TI const* src = static_cast<TI const*>(p.v) + (int64_t)row * p.v_stride[0] + (int64_t)hv * p.v_stride[1];
-                    TC*       dst = vc + (int64_t)hv * p.vc_stride[2];
-                    uint32_t const e = 8 * u;
-                    if (e < p.d) {
-                        float     x[8];
-                        int const n = min(8, (int)(p.d - e));
-                        load_n<8, VEC>(src + e, x, n);
-                        store_n<8, VEC>(dst + e, x, n);
-                    }
-                }
+        TI const* s = src;
+        TC*       d = dst + at.to;
+        for (uint32_t h = h0; h < heads; h += 2 * at_once) { // two heads' loads in flight, beside the angles'
+            bool const two = h + at_once < heads;
+            raw_t<TI>  in[2];
+            load_unit<HALVES, VEC>(s, t, in[0]);
+            if (two) load_unit<HALVES, VEC>(s + at_once * si1, t, in[1]);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                if (x && !two) break;
+                TC* const to = d + (x ? at_once * so1 : 0);
+                float     y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = to_f32(in[x].v[j]);
+                if (turn) rotate<HALVES>(y, c);
+                store_unit<HALVES, VEC>(to, t, y);
             }
+            s += 2 * at_once * si1;
+            d += 2 * at_once * so1;
         }
     }
 }
@@ -291,10 +339,9 @@ int launch_cache_append(es_cache_append_t const& a, es_cache_append_args_t const
     p.page = make_fastdivide(c.page_size);
     bool const     halves = a.pairing == ES_ROPE_HALVES && a.rotary_dim > 0;
     uint32_t const half = a.rotary_dim / 2;
-    // threads a head: adjacent pairs ceil(d / 8); halves: runs of 4 of either half, then 8 of the rest (and at
-    // least ceil(d / 8) for the values)
-    p.units_per_head = halves ? std::max((half + 3) / 4 + (c.head_dim - a.rotary_dim + 7) / 8, (c.head_dim + 7) / 8) : (c.head_dim + 7) / 8;
-    p.upd = make_fastdivide(p.units_per_head);
+    // units a head: adjacent pairs ceil(d / 8); halves: runs of 4 of either half, then 8 of the rest
+    uint32_t const units = halves ? (half + 3) / 4 + (c.head_dim - a.rotary_dim + 7) / 8 : (c.head_dim + 7) / 8;
+    p.upd = make_fastdivide(units);
     // 16-byte accesses when every run of 8 (with halves: 4) elements of every head starts on its own size
     uint64_t  bits = reinterpret_cast<uintptr_t>(x.k) | reinterpret_cast<uintptr_t>(x.v) | reinterpret_cast<uintptr_t>(x.k_cache) |
                      reinterpret_cast<uintptr_t>(x.v_cache) | reinterpret_cast<uintptr_t>(x.freqs);
@@ -307,16 +354,24 @@ int launch_cache_append(es_cache_append_t const& a, es_cache_append_args_t const
     }
     el |= a.rotary_dim; // a multiple of 8: a row of angles is a multiple of 32 bytes, a half of 4 elements
     bool const vec = (bits & 15) == 0 && (el & 7) == 0;
-    // A block a row; when the rows alone would leave SMs empty (under 2 blocks an SM) a row's heads are shared
-    // out to up to 16 blocks of fewer threads.
-    uint32_t const units = (a.heads + 2 * c.kv_heads) * p.units_per_head;
-    uint32_t const want = std::max<uint32_t>(1, (2 * SM_COUNT + c.rows - 1) / c.rows);
-    uint32_t       threads = 256;
-    while (threads > 64 && (units + threads - 1) / threads < want) threads /= 2;
-    uint32_t const gy = std::min<uint32_t>(std::min<uint32_t>(want, 16), (units + threads - 1) / threads);
-    dim3 const     grid(std::min<uint32_t>(c.rows, 1u << 20), gy);
-    auto           go = [&](auto kernel) { launch_k(kernel, grid, dim3(threads), 0, stream, p); };
-    auto           pick = [&](auto ti, auto tc) {
+    // one wave of blocks, the same number of units each
+    p.by_heads[0] = make_fastdivide(std::max(a.heads, 1u));
+    p.by_heads[1] = make_fastdivide(c.kv_heads);
+    uint64_t const wave = blocks_an_sm(a.in_dtype == ES_F16 && vec) * SM_COUNT;
+    uint64_t const all = (uint64_t)c.rows * (a.heads + 2ull * c.kv_heads) * units;
+    uint64_t const share = std::max<uint64_t>(APPEND_THREADS, (all + wave - 1) / wave);
+    auto           rows_for = [&](uint64_t a_row) { return (uint32_t)std::min<uint64_t>(ROWS_MAX, std::max<uint64_t>(1, (share + a_row - 1) / a_row)); };
+    p.rows_a_block[0] = rows_for((uint64_t)std::max(a.heads, 1u) * units);
+    p.rows_a_block[1] = rows_for((uint64_t)c.kv_heads * units);
+    uint64_t const bq = a.heads ? (c.rows + (uint64_t)p.rows_a_block[0] - 1) / p.rows_a_block[0] : 0;
+    uint64_t const bk = (c.rows + (uint64_t)p.rows_a_block[1] - 1) / p.rows_a_block[1];
+    if (bq + 2 * bk > 0x7fffffffull) fail(ES_NOT_SUPPORTED, "cache append: too many rows");
+    p.first_block[0] = (uint32_t)bq;
+    p.first_block[1] = (uint32_t)(bq + bk);
+    dim3 const  grid((uint32_t)(bq + 2 * bk));
+    pdl_scope_t scope(true); // (the kernel waits for those before it itself)
+    auto        go = [&](auto kernel) { launch_k(kernel, grid, dim3(APPEND_THREADS), 0, stream, p); };
+    auto        pick = [&](auto ti, auto tc) {
         using TI = decltype(ti);
         using TC = decltype(tc);
         if (vec) {

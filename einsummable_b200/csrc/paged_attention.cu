@@ -114,10 +114,9 @@ uint64_t most_keys(paged_params_t const& p)
     return p.prefix_len >= 0 ? (uint64_t)p.prefix_len : (uint64_t)p.capacity + p.front;
 }
 
-template <typename T, int NCH, bool VEC> part_t simt_as(paged_params_t p)
+template <typename T, int NCH, int TR, bool VEC> part_t simt_as(paged_params_t p)
 {
-    constexpr uint32_t TR = 16 / NCH;
-    part_t             c;
+    part_t c;
     p.part_d = NCH * 32;
     // Direct: with at most 8 key tiles an item, one block an item and no join -- a join costs as much as
     // about 8 tiles take
@@ -125,7 +124,7 @@ template <typename T, int NCH, bool VEC> part_t simt_as(paged_params_t p)
     c.p = p;
     c.main = [](paged_params_t const& p, cudaStream_t s) {
         dim3 const grid(p.direct ? p.kv_heads * ((p.group + TR - 1) / TR) : SIMT_BLOCKS, p.direct ? p.batch : 1);
-        launch_k(paged_simt_kernel<T, NCH, VEC>, grid, dim3(128), 0, s, p);
+        launch_k(paged_simt_kernel<T, NCH, TR, VEC>, grid, dim3(128), 0, s, p);
     };
     c.join = nullptr;
     if (!p.direct)
@@ -134,11 +133,29 @@ template <typename T, int NCH, bool VEC> part_t simt_as(paged_params_t p)
         };
     return c;
 }
+// TR: rows that read a key together: as many as there are for one token, up to what fits the registers
+template <typename T, bool VEC> part_t simt_part(paged_params_t const& p)
+{
+    bool const one = sizeof(T) == 4 && p.group == 1 && !p.row_offsets && p.prefix_len < 0;
+    if (p.d <= 64) {
+        if constexpr (sizeof(T) == 4) {
+            if (one) return simt_as<T, 2, 1, VEC>(p);
+            if (p.group > 4) return simt_as<T, 2, 8, VEC>(p);
+        }
+        return simt_as<T, 2, 4, VEC>(p);
+    }
+    if (p.d <= 128) {
+        if constexpr (sizeof(T) == 4)
+            if (one) return simt_as<T, 4, 1, VEC>(p);
+        return simt_as<T, 4, 4, VEC>(p);
+    }
+    if constexpr (sizeof(T) == 4)
+        if (one) return simt_as<T, 8, 1, VEC>(p);
+    return simt_as<T, 8, 2, VEC>(p);
+}
 template <typename T> part_t simt_part(paged_params_t const& p, bool vec)
 {
-    if (p.d <= 64) return vec ? simt_as<T, 2, true>(p) : simt_as<T, 2, false>(p);
-    if (p.d <= 128) return vec ? simt_as<T, 4, true>(p) : simt_as<T, 4, false>(p);
-    return vec ? simt_as<T, 8, true>(p) : simt_as<T, 8, false>(p);
+    return vec ? simt_part<T, true>(p) : simt_part<T, false>(p);
 }
 
 // Kernels with more shared memory than 48 KB say so once per device
@@ -323,8 +340,7 @@ int launch_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
     uint64_t const all = (uint64_t)c.batch * a.prefix_len * c.kv_heads * c.head_dim * 2 * dtype_size(c.dtype);
     bool const     front = a.prefix_len && !x.row_offsets && p.group <= MMA_MAX_TR && all <= (64ull << 20);
     int            launches = 0;
-    bool const     pdl = pdl_launch_flag();
-    auto           next = [&] { return pdl_scope_t(launches++ > 0 || pdl); };
+    pdl_scope_t    scope(true); // (every kernel waits for those before it itself)
     if (front) {
         p.front = a.prefix_len;
         p.front_pages = x.prefix_pages;
@@ -341,14 +357,9 @@ int launch_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
         for (int i = 0; i != n; ++i) {
             use_region(k[i].p, ws, l.region[0]);
             k[i].p.order = i == 0 && n == 1 ? ORDER_FIRST : ORDER_PLAIN;
-            {
-                auto scope = next();
-                k[i].main(k[i].p, stream);
-            }
-            if (k[i].join) {
-                auto scope = next();
-                k[i].join(k[i].p, stream);
-            }
+            k[i].main(k[i].p, stream);
+            if (k[i].join) k[i].join(k[i].p, stream);
+            launches += k[i].join ? 2 : 1;
         }
         // the sequences' own keys need the prefix's result only where a row is finished
         p.order = n == 1 ? ORDER_LATE : ORDER_PLAIN;
@@ -365,14 +376,11 @@ int launch_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
     }
     for (int i = 0; i != n; ++i) {
         use_region(k[i].p, ws, l.region[n == 2 ? i : 1]);
-        auto scope = next();
         k[i].main(k[i].p, stream);
+        launches += k[i].join ? 2 : 1;
     }
-    for (int i = 0; i != n; ++i) {
-        if (!k[i].join) continue;
-        auto scope = next();
-        k[i].join(k[i].p, stream);
-    }
+    for (int i = 0; i != n; ++i)
+        if (k[i].join) k[i].join(k[i].p, stream);
     return launches;
 }
 

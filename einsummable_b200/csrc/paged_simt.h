@@ -4,8 +4,10 @@
 // 8 lanes hold one key's head dim (4 elements at a time, 32 elements apart); a block's 16 such groups each
 // take every 16th key and keep running maxima, sums and results of their own for TR rows, so that nothing is
 // exchanged between groups until the segment ends.  The query rows stay in registers, multiplied by
-// scale * log2 e.  The next key and value are loaded before the current ones are used.  Bound: memory for up
-// to TR packed rows a key head; beyond that a key is read once per TR rows.
+// scale * log2 e.  The next KEYS keys and values are loaded before the current ones are used.  Bound: the latency
+// of those loads for short sequences, memory for long ones with up to TR packed rows a key head; beyond that a key
+// is read once per TR rows.  TR follows the rows there are (12 sequences of up to 2900 tokens, 4 query heads of 64
+// a key head: 17 us with 8 rows and one key at a time).
 #pragma once
 #include "paged_work.h"
 
@@ -33,10 +35,11 @@ template <typename T> __device__ __forceinline__ void load4(T const* p, float (&
     }
 }
 
-template <typename T, int NCH, bool VEC> // NCH: chunks of 32 elements of the head dim
+template <typename T, int NCH, int TR, bool VEC> // NCH: chunks of 32 elements of the head dim
 __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__ paged_params_t p)
 {
-    constexpr int TR = 16 / NCH, BK = SIMT_BK, OVH = SIMT_OVH, NT = 128;
+    constexpr int KEYS = NCH * TR <= 8 && NCH <= 4 ? 2 : 1, BK = SIMT_BK, OVH = SIMT_OVH, NT = 128;
+    constexpr bool AHEAD = NCH <= 4; // (head dims above 128: no registers for it)
     __shared__ sched_smem_t<NT, 1> sched;
     __shared__ float            so[4][TR][NCH * 32];
     __shared__ float2           sml[4][TR];
@@ -102,51 +105,70 @@ __global__ void __launch_bounds__(128) paged_simt_kernel(const __grid_constant__
             }
             return true;
         };
-        float     k[NCH][4], v[NCH][4];
+        float     k[KEYS][NCH][4], v[KEYS][NCH][4];
+        bool      have[KEYS];
         int const key0 = key_begin + stream;
-        bool      have = load(key0, k, v);
+#pragma unroll
+        for (int x = 0; x < KEYS; ++x) have[x] = load(key0 + x * 16, k[x], v[x]);
         // (every group of the warp makes the same number of rounds: the shuffles are the warp's)
-        int const rounds = key_end > key_begin ? (key_end - key_begin + 15) / 16 : 0;
+        int const rounds = key_end > key_begin ? (key_end - key_begin + 16 * KEYS - 1) / (16 * KEYS) : 0;
         for (int i = 0; i < rounds; ++i) {
-            int const key = key0 + i * 16;
-            float     kn[NCH][4], vn[NCH][4];
-            bool const next = i + 1 < rounds && load(key + 16, kn, vn);
+            int const key = key0 + i * 16 * KEYS;
+            float     kn[KEYS][NCH][4], vn[KEYS][NCH][4];
+            bool      next[KEYS];
+#pragma unroll
+            for (int x = 0; x < KEYS; ++x) next[x] = AHEAD && i + 1 < rounds && load(key + (KEYS + x) * 16, kn[x], vn[x]);
 #pragma unroll
             for (int r = 0; r < TR; ++r) {
-                float s = 0.f;
+                float s[KEYS];
 #pragma unroll
-                for (int c = 0; c < NCH; ++c)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) s = fmaf(q[r][c][x], k[c][x], s);
-                s += __shfl_xor_sync(0xffffffffu, s, 4);
-                s += __shfl_xor_sync(0xffffffffu, s, 2);
-                s += __shfl_xor_sync(0xffffffffu, s, 1);
-                if (have && key - own < vis[r]) {
-                    if (s > m[r]) {
-                        float const a = ex2(m[r] - s); // m = -inf: 0
-                        m[r] = s;
-                        l[r] *= a;
-#pragma unroll
-                        for (int c = 0; c < NCH; ++c)
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) o[r][c][x] *= a;
-                    }
-                    float const e = ex2(s - (m[r] == -INFINITY ? 0.f : m[r]));
-                    l[r] += e;
+                for (int x = 0; x < KEYS; ++x) {
+                    s[x] = 0.f;
 #pragma unroll
                     for (int c = 0; c < NCH; ++c)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) o[r][c][x] = fmaf(e, v[c][x], o[r][c][x]);
+                        for (int y = 0; y < 4; ++y) s[x] = fmaf(q[r][c][y], k[x][c][y], s[x]);
+                }
+#pragma unroll
+                for (int d = 4; d; d >>= 1)
+#pragma unroll
+                    for (int x = 0; x < KEYS; ++x) s[x] += __shfl_xor_sync(0xffffffffu, s[x], d);
+#pragma unroll
+                for (int x = 0; x < KEYS; ++x) {
+                    if (have[x] && key + x * 16 - own < vis[r]) {
+                        if (s[x] > m[r]) {
+                            float const a = ex2(m[r] - s[x]); // m = -inf: 0
+                            m[r] = s[x];
+                            l[r] *= a;
+#pragma unroll
+                            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                                for (int y = 0; y < 4; ++y) o[r][c][y] *= a;
+                        }
+                        float const e = ex2(s[x] - (m[r] == -INFINITY ? 0.f : m[r]));
+                        l[r] += e;
+#pragma unroll
+                        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) o[r][c][y] = fmaf(e, v[x][c][y], o[r][c][y]);
+                    }
                 }
             }
-            have = next;
 #pragma unroll
-            for (int c = 0; c < NCH; ++c)
+            for (int x = 0; x < KEYS; ++x) {
+                if constexpr (AHEAD) {
+                    have[x] = next[x];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    k[c][x] = kn[c][x];
-                    v[c][x] = vn[c][x];
+                    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            k[x][c][y] = kn[x][c][y];
+                            v[x][c][y] = vn[x][c][y];
+                        }
+                } else {
+                    have[x] = i + 1 < rounds && load(key + (KEYS + x) * 16, k[x], v[x]);
                 }
+            }
         }
         // the warp's four groups
 #pragma unroll

@@ -4,30 +4,33 @@
 // Bound: the tensor cores, and as much the exponentials: a tile of 128 rows x 128 keys of 128 elements is 2 * 512
 // cycles of products and, at 16 exponentials a cycle, 1024 of softmax.  So an item is two tiles of 128 packed rows
 // that share the keys in shared memory and take turns: while one tile's scores are on the tensor cores, the
-// other's are exponentials.  One persistent block an SM, 12 warps:
-//   warps 0-3, 4-7   softmax of tile 0 / 1, a thread a row (= TMEM lane): maximum of the 128 scores, rescaling of
-//                    the accumulator when it has moved by more than 2^8, exponentials (f32; rounded to f16 for
-//                    the product with the values), written as f16 pairs over the scores they came from; and the
-//                    copies of the tile's queries, those of the next item as soon as the last scores are there
-//   warp 8           issues the products: S_t = Q_t K^T into TMEM, O_t += P_t V with P_t read from TMEM
-//   warps 9-11       copy the pages into the 128-byte-swizzled tiles the tensor cores read, 16 keys of one page at a
+// other's are exponentials.  One persistent block an SM, 20 warps:
+//   warps 0-7, 8-15  softmax of tile 0 / 1, two threads a row (= TMEM lane), 64 keys each -- with one thread a row the
+//                    chain scores, maximum, 128 exponentials, products took 3500 cycles a tile: maximum of the
+//                    scores, rescaling of the accumulator when it has moved by more than 2^8, exponentials (f32;
+//                    rounded to f16 for the product with the values), written as f16 pairs over the scores they
+//                    came from; and the copies of the tile's queries, those of the next item as soon as the last
+//                    scores are there
+//   warp 16          issues the products: S_t = Q_t K^T into TMEM, O_t += P_t V with P_t read from TMEM
+//   warps 17-19      copy the pages into the 128-byte-swizzled tiles the tensor cores read, 16 keys of one page at a
 //                    time (a warp every third 16; one by one where pages are no multiple of 16 tokens, and in the
 //                    sequence's last tile); page numbers are fetched a tile ahead; two stages each for keys and
 //                    values.  (With every row's address sent through a shuffle a tile's 64 KB took 8700 cycles.)
 // TMEM: scores 2 x 128 columns, accumulators 2 x 128.  Products of one thread are done in order, so S_t of the
 // next tile may be issued over P_t as soon as P_t V is, and whoever sees S_t complete knows P_t V to be.
-// Every wait is bounded; on expiry the kernel records 0x31-0x38, lets its copies land, frees TMEM and returns.
+// Every wait is bounded; on expiry the kernel records 0x31-0x39, lets its copies land, frees TMEM and returns.
 #pragma once
 #include "paged_mma.h"
 
 namespace es {
 namespace {
 
-constexpr int      WIDE_TR = 256, WIDE_BK = 128, WIDE_OVH = 4, WIDE_COPY_WARPS = 3, WIDE_THREADS = (9 + WIDE_COPY_WARPS) * 32;
+constexpr int      WIDE_TR = 256, WIDE_BK = 128, WIDE_OVH = 4, WIDE_SOFTMAX_WARPS = 16, WIDE_COPY_WARPS = 3,
+                   WIDE_THREADS = (WIDE_SOFTMAX_WARPS + 1 + WIDE_COPY_WARPS) * 32;
 constexpr uint64_t WIDE_WAIT_LIMIT_CYCLES = 4000000000ull; // ~2 s at 2 GHz
 
 struct wide_ctrl_t {
-    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], o_free[2];
+    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], o_free[2], pair[8];
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
@@ -58,19 +61,16 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
 }
-// 32 columns of this thread's lane, there after tcgen05.wait::ld
-__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r)
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
 {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, uint32_t const (&r)[16])
 {
@@ -82,10 +82,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, uint32_t const (&r)[16
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_wait_ld()
-{
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
 // two f32 at a time
 __device__ __forceinline__ uint64_t pack2(float lo, float hi)
 {
@@ -116,7 +112,7 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return r;
 }
 
-constexpr uint32_t WIDE_STAGE_BYTES = 8 * 2048; // results on their way out: 32 rows of 32 f16 a warp
+constexpr uint32_t WIDE_STAGE_BYTES = WIDE_SOFTMAX_WARPS * 1024; // results on their way out: 32 rows of 16 f16 a warp
 template <int DPAD> constexpr uint32_t wide_smem_bytes()
 {
     return 6 * (DPAD / 64) * 16384 + WIDE_STAGE_BYTES + (uint32_t)sizeof(wide_ctrl_t) + 1024;
@@ -128,6 +124,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
     constexpr int      TR = WIDE_TR, BK = WIDE_BK, OVH = WIDE_OVH;
     constexpr uint32_t KB = DPAD / 64, BLOCK = 16384, TILE = KB * BLOCK; // 64-element blocks: 128 rows of 128 bytes
     __shared__ sched_smem_t<WIDE_THREADS, 1> sched;
+    __shared__ float                         row_value[2][2][2][128]; // what a row's two threads tell one another: [turn][tile][half][row]
     extern __shared__ uint8_t                smem_wide[];
     uint8_t* const     smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_wide) + 1023) & ~uintptr_t(1023));
     wide_ctrl_t* const ctrl = reinterpret_cast<wide_ctrl_t*>(smem + 6 * TILE + WIDE_STAGE_BYTES);
@@ -136,24 +133,26 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
     uint32_t const     bars = smem_u32(ctrl);
     // in the order of wide_ctrl_t
     uint32_t const     q_full = bars, k_full = q_full + 16, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16, s_full = v_empty + 16,
-                   p_ready = s_full + 16, o_done = p_ready + 16, o_free = o_done + 16;
+                   p_ready = s_full + 16, o_done = p_ready + 16, o_free = o_done + 16,
+                   pair = o_free + 16;
     int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(q_full + 8 * i, 128);
+            mbar_init(q_full + 8 * i, 256);
             mbar_init(k_full + 8 * i, WIDE_COPY_WARPS * 32);
             mbar_init(k_empty + 8 * i, 1);
             mbar_init(v_full + 8 * i, WIDE_COPY_WARPS * 32);
             mbar_init(v_empty + 8 * i, 1);
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_ready + 8 * i, 128);
+            mbar_init(p_ready + 8 * i, 256);
             mbar_init(o_done + 8 * i, 1);
-            mbar_init(o_free + 8 * i, 128);
+            mbar_init(o_free + 8 * i, 256);
         }
+        for (int i = 0; i < 8; ++i) mbar_init(pair + 8 * i, 64);
         ctrl->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == WIDE_SOFTMAX_WARPS) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctrl->tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -169,10 +168,10 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
     work_t w;
     find_work<TR, BK, OVH, WIDE_THREADS, 1>(p, w, sched);
 
-    if (warp >= 9) {
+    if (warp > WIDE_SOFTMAX_WARPS) {
         // ------------------------------------------------------------ copies of keys and values
         constexpr int  CH = DPAD / 8, ROWS_AT = 32 / CH, STEPS = 16 / ROWS_AT;
-        int const      lw = warp - 9, c_row = lane / CH, c_chunk = lane % CH;
+        int const      lw = warp - WIDE_SOFTMAX_WARPS - 1, c_row = lane / CH, c_chunk = lane % CH;
         bool const     c_on = (uint32_t)c_chunk * 8 < p.d;
         // chunk c of row r lies in block c / 8 at chunk (c % 8) ^ (r % 8)
         uint32_t const c_dst = (uint32_t)(c_chunk >> 3) * BLOCK + c_row * 128 + (((c_chunk & 7) ^ c_row) << 4);
@@ -264,7 +263,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
             next_item<TR, BK, OVH>(p, w, n);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp == 8) {
+    } else if (warp == WIDE_SOFTMAX_WARPS) {
         // ------------------------------------------------------------ products (the whole warp; one lane issues)
         bool leader;
         {
@@ -294,8 +293,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
             uint32_t const d = tmem + 256 + t * 128, a = tmem + t * 128;
             if (leader) {
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) // 16 keys a product: 8 TMEM columns of P, 16 rows of V
-                    umma_ts(d, a + i * 8, b + (uint64_t)((i * 2048) >> 4), idesc_o, (keep || i) ? 1u : 0u);
+                for (uint32_t i = 0; i < 8; ++i) // 16 keys a product: 8 TMEM columns of P (over the scores of its 64 keys), 16 rows of V
+                    umma_ts(d, a + (i >> 2) * 64 + (i & 3) * 8, b + (uint64_t)((i * 2048) >> 4), idesc_o, (keep || i) ? 1u : 0u);
             }
         };
         auto commit = [&](uint32_t b) {
@@ -344,25 +343,35 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
             next_item<TR, BK, OVH>(p, w, n);
         }
     } else {
-        // ------------------------------------------------------------ softmax: a thread a row
-        uint32_t const t = warp >> 2, r_tile = threadIdx.x & 127;
-        uint32_t const row_s = tmem + t * 128 + ((uint32_t)((warp & 3) * 32) << 16);
-        uint32_t const row_o = row_s + 256;
-        uint32_t       n_s = 0, n_o = 0;
+        // ------------------------------------------------------------ softmax: two threads a row
+        constexpr int  OH = DPAD / 2; // columns of the accumulator that a thread looks after
+        uint32_t const t = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, r_tile = quarter * 32 + lane;
+        uint32_t const lanes = (uint32_t)(quarter * 32) << 16;
+        uint32_t const row_s = tmem + t * 128 + half * 64 + lanes, row_o = tmem + 256 + t * 128 + half * OH + lanes;
+        uint32_t       n_s = 0, n_o = 0, turn = 0;
         bool           ok = true, split = false;
-        // this warp's 32 query rows of an item's tile t (none if the item has no key tile here); tell_q follows
+        // x becomes the other thread's value (the two warps of a quarter meet)
+        auto exchange = [&](float& x) {
+            row_value[turn][t][half][r_tile] = x;
+            mbar_arrive(pair + 8 * (t * 4 + quarter));
+            bool const met = __all_sync(0xffffffffu, wide_wait(p, pair + 8 * (t * 4 + quarter), turn, abort_flag, 0x39)) != 0;
+            x = row_value[turn][t][half ^ 1][r_tile];
+            turn ^= 1; // (a value is overwritten two meetings later)
+            return met;
+        };
+        // this warp's 16 query rows of an item's tile t (none if the item has no key tile here); tell_q follows
         auto load_q = [&](work_t const& x) -> bool {
             if (x.left == 0) return false;
             uint32_t const n = min(x.kt - x.j, x.left), start = x.t * TR, count = min((uint32_t)TR, (uint32_t)x.s.n * p.group - start);
             if (first_tile_of<OVH>(x.j + n) == first_tile_of<OVH>(x.j) || t * 128 >= count) return false;
             constexpr int  CH = DPAD / 8, ROWS_AT = 32 / CH;
-            uint32_t const first = t * 128 + (warp & 3) * 32;
-            uint32_t const pr = start + min(first + lane, count - 1), tok = fdivide(pr, p.grp);
+            uint32_t const first = t * 128 + quarter * 32 + half * 16;
+            uint32_t const pr = start + min(first + (lane & 15), count - 1), tok = fdivide(pr, p.grp);
             int64_t const  mine = (int64_t)(x.s.row0 + (int)tok) * p.q_stride[0] + (int64_t)(x.head * p.group + (pr - tok * p.group)) * p.q_stride[1];
             uint32_t const c_row = lane / CH, c = lane % CH;
             __half const*  q = static_cast<__half const*>(p.q) + c * 8;
 #pragma unroll 4
-            for (int i = 0; i < 32 / ROWS_AT; ++i) {
+            for (int i = 0; i < 16 / ROWS_AT; ++i) {
                 uint32_t const r = c_row + i * ROWS_AT, row = (first & 127) + r;
                 int64_t const  at = __shfl_sync(0xffffffffu, mine, r);
                 if (c * 8 < p.d) copy16(sQ + t * TILE + (c >> 3) * BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4), q + at, first + r < count);
@@ -388,7 +397,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
             bool const here = t * 128 < count && f1 > f0; // this warp has rows and keys in the item
             if (!here && load_next_q()) tell_q();
             if (t * 128 < count) {
-                float          m = MMA_NO_KEY, l = 0.f;
+                float          m = MMA_NO_KEY, l = 0.f; // l: of this thread's keys
                 uint32_t const pr = start + min(r, count - 1), tok = fdivide(pr, p.grp);
                 int const      vis = visible(p, w.s, (int)tok);
                 for (uint32_t j = f0; j < f1; ++j) {
@@ -398,11 +407,10 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     tc_fence_after();
                     // every product with this item's queries is done: the next item's may come
                     bool const more = j + 1 == f1 && load_next_q();
-                    int const  allow = vis - (int)(j * BK); // this row sees the tile's first `allow` keys
-                    bool const mask = __any_sync(0xffffffffu, allow < BK);
-                    // Scores are read 64 at a time (128 at once do not fit beside the rest): the maximum of the second
-                    // half, then of the first, which stays for its exponentials; P of the first half may then lie over
-                    // it, and the second half is read again.
+                    int const  allow = vis - (int)(j * BK + half * 64); // this row sees the first `allow` of the thread's keys
+                    bool const mask = __any_sync(0xffffffffu, allow < 64);
+                    // The scores are read twice, 32 at a time (there are 96 registers): for the maximum, the second half
+                    // first, and for the exponentials, so that P of the first half may lie over scores that have been read.
                     auto hide = [&](uint32_t (&v)[32], int first) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
@@ -413,38 +421,29 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
                     };
-                    uint32_t x0[32], x1[32];
-                    tmem_ld32_async(row_s + 64, x0);
-                    tmem_ld32_async(row_s + 96, x1);
-                    tmem_wait_ld();
-                    if (mask) {
-                        hide(x0, 64);
-                        hide(x1, 96);
-                    }
-                    largest(x0);
-                    largest(x1);
-                    tmem_ld32_async(row_s, x0);
-                    tmem_ld32_async(row_s + 32, x1);
-                    tmem_wait_ld();
-                    if (mask) {
-                        hide(x0, 0);
-                        hide(x1, 32);
-                    }
-                    largest(x0);
-                    largest(x1);
-                    float const top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;
-                    if (__any_sync(0xffffffffu, top > m + MMA_RESCALE)) {
+                    uint32_t x[32];
+                    tmem_ld32(row_s + 32, x);
+                    if (mask) hide(x, 32);
+                    largest(x);
+                    tmem_ld32(row_s, x);
+                    if (mask) hide(x, 0);
+                    largest(x);
+                    float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+                    float others = top;
+                    if (!(ok = exchange(others))) break;
+                    top = fmaxf(top, others) * p.scale_log2;
+                    if (__any_sync(0xffffffffu, top > m + MMA_RESCALE)) { // (the same in both warps)
                         float const mn = fmaxf(m, top), a = ex2(m - mn);
                         m = mn;
                         l *= a;
                         if (j != f0) {
 #pragma unroll 1
-                            for (int c = 0; c < DPAD / 32; ++c) {
-                                uint32_t o[32];
-                                tmem_ld32(row_o + c * 32, o);
+                            for (int c = 0; c < OH / 16; ++c) {
+                                uint32_t o[16];
+                                tmem_ld16(row_o + c * 16, o);
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-                                tmem_st32(row_o + c * 32, o);
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+                                tmem_st16(row_o + c * 16, o);
                             }
                         }
                     }
@@ -463,16 +462,10 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                         }
                         tmem_st16(row_s + c * 16, y);
                     };
-                    exponentials(x0, 0);
-                    tmem_ld32_async(row_s + 64, x0);
-                    exponentials(x1, 1);
-                    tmem_wait_ld();
-                    tmem_ld32_async(row_s + 96, x1);
-                    if (mask) hide(x0, 64);
-                    exponentials(x0, 2);
-                    tmem_wait_ld();
-                    if (mask) hide(x1, 96);
-                    exponentials(x1, 3);
+                    exponentials(x, 0);
+                    tmem_ld32(row_s + 32, x);
+                    if (mask) hide(x, 32);
+                    exponentials(x, 1);
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                     mbar_arrive(p_ready + 8 * t);
@@ -482,6 +475,9 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     if (more) tell_q();
                 }
                 if (!ok) break;
+                float others = l;
+                if (!(ok = exchange(others))) break;
+                l = half ? others + l : l + others; // (the same sum in both)
                 if (f1 > f0) {
                     ok = __all_sync(0xffffffffu, wide_wait(p, o_done + 8 * t, n_o & 1, abort_flag, 0x36)) != 0;
                     if (!ok) break;
@@ -495,40 +491,41 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                 if (to < 0 && p.base_out) wait_for_base(p);
                 if (to < 0 && r < count) {
                     f = finish(m, l, p.base_lse != nullptr, p.base_lse ? p.base_lse[at] : 0.f);
-                    if (p.lse) p.lse[at] = f.lse;
+                    if (p.lse && half == 0) p.lse[at] = f.lse;
                 }
-                if (to >= 0 && r < count) p.part_ml[part] = make_float2(m, l);
+                if (to >= 0 && r < count && half == 0) p.part_ml[part] = make_float2(m, l);
                 bool const staged = to < 0 && !p.out_f32; // f16 rows go out through shared memory
-                __half*    dst[4] = {};                   // row (lane / 4) + 8 i of the warp's 32, elements 8 (lane % 4) ..
+                __half*    dst[2] = {};                   // row lane / 2 + 16 i of the warp's 32, elements 8 (lane % 2) ..
                 if (staged) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t const rw = t * 128 + (warp & 3) * 32 + (lane >> 2) + 8 * i;
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t const rw = t * 128 + quarter * 32 + (lane >> 1) + 16 * i;
                         uint32_t const q = start + min(rw, count - 1), qt = fdivide(q, p.grp);
                         if (rw < count)
                             dst[i] = static_cast<__half*>(p.out) + (int64_t)(w.s.row0 + (int)qt) * p.out_stride[0] +
-                                     (int64_t)(w.head * p.group + (q - qt * p.group)) * p.out_stride[1] + (lane & 3) * 8;
+                                     (int64_t)(w.head * p.group + (q - qt * p.group)) * p.out_stride[1] + half * OH + (lane & 1) * 8;
                     }
                 }
-                uint32_t const stage = sQ + 6 * TILE + warp * 2048;
+                uint32_t const stage = sQ + 6 * TILE + warp * 1024;
 #pragma unroll 1
-                for (int c = 0; c < DPAD / 32; ++c) {
-                    uint32_t x[32];
+                for (int c = 0; c < OH / 16; ++c) {
+                    uint32_t const e = half * OH + c * 16; // of the head dim (a multiple of 8)
+                    uint32_t       x[16];
                     if (f1 > f0) {
-                        tmem_ld32(row_o + c * 32, x);
+                        tmem_ld16(row_o + c * 16, x);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = 0;
+                        for (int i = 0; i < 16; ++i) x[i] = 0;
                     }
                     if (staged) {
-                        float v[32];
+                        float v[16];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = f.wa == 0.f ? 0.f : __uint_as_float(x[i]) * f.wa; // a weight of 0: the sum may be anything
+                        for (int i = 0; i < 16; ++i) v[i] = f.wa == 0.f ? 0.f : __uint_as_float(x[i]) * f.wa; // a weight of 0: the sum may be anything
                         if (f.wb != 0.f) {
-                            float const* base = p.base_out + at * p.d + c * 32;
+                            float const* base = p.base_out + at * p.d + e;
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4) {
-                                if ((uint32_t)(c * 32 + i) < p.d) { // (the head dim is a multiple of 8)
+                            for (int i = 0; i < 16; i += 4) {
+                                if (e + i < p.d) {
                                     float4 const b = *reinterpret_cast<float4 const*>(base + i);
                                     v[i] = fmaf(b.x, f.wb, v[i]);
                                     v[i + 1] = fmaf(b.y, f.wb, v[i + 1]);
@@ -539,28 +536,28 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                         }
                         __syncwarp(); // the chunk before has been read
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) // 16 bytes; four rows share 128 bytes' worth of banks twice
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)),
+                        for (int i = 0; i < 2; ++i)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 32 + ((i ^ ((lane >> 2) & 1)) << 4)),
                                          "r"(pack_h2(v[8 * i], v[8 * i + 1])), "r"(pack_h2(v[8 * i + 2], v[8 * i + 3])),
                                          "r"(pack_h2(v[8 * i + 4], v[8 * i + 5])), "r"(pack_h2(v[8 * i + 6], v[8 * i + 7])) : "memory");
                         __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t const rw = (lane >> 2) + 8 * i;
+                        for (int i = 0; i < 2; ++i) {
+                            uint32_t const rw = (lane >> 1) + 16 * i;
                             uint4          y;
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
-                                         : "r"(stage + rw * 64 + (((lane & 3) ^ ((rw >> 1) & 3)) << 4)) : "memory");
-                            if (dst[i] && (uint32_t)(c * 32 + (lane & 3) * 8) < p.d) *reinterpret_cast<uint4*>(dst[i] + c * 32) = y;
+                                         : "r"(stage + rw * 32 + (((lane & 1) ^ ((rw >> 2) & 1)) << 4)) : "memory");
+                            if (dst[i] && e + (lane & 1) * 8 < p.d) *reinterpret_cast<uint4*>(dst[i] + c * 16) = y;
                         }
                     } else if (r < count) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
+                        for (int i = 0; i < 16; i += 4) {
                             float const v4[4] = {__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])};
                             if (to < 0) {
-                                if ((uint32_t)(c * 32 + i) < p.d) write_out<__half, 4>(p, row, head, c * 32 + i, v4, f, true);
+                                if (e + i < p.d) write_out<__half, 4>(p, row, head, e + i, v4, f, true);
                             } else {
                                 // four elements of 256 rows, then the next four: a warp's store is one run of 512 bytes
-                                *reinterpret_cast<float4*>(p.part_out + (uint64_t)(2 * w.worker + to) * TR * DPAD + ((c * 8 + i / 4) * TR + r) * 4) =
+                                *reinterpret_cast<float4*>(p.part_out + (uint64_t)(2 * w.worker + to) * TR * DPAD + (((e + i) / 4) * TR + r) * 4) =
                                     make_float4(v4[0], v4[1], v4[2], v4[3]);
                             }
                         }
@@ -587,7 +584,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
         __syncthreads();
     }
-    if (warp == 8) {
+    if (warp == WIDE_SOFTMAX_WARPS) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
@@ -601,10 +598,10 @@ template <int DPAD> __global__ void __launch_bounds__(256) paged_wide_join_kerne
     constexpr int    TR = WIDE_TR, CH = DPAD / 64; // chunks of 64 elements, 4 a thread
     __shared__ float so[16][DPAD + 4];
     ES_PDL_PROLOGUE();
-    int4 const     m0 = p.meta[2 * blockIdx.x];
+    int4 const     m0 = p.meta[2 * blockIdx.x], m1 = p.meta[2 * blockIdx.x + 1]; // (m1 means something if m0.x > 0)
     uint32_t const r0 = blockIdx.y * 16;
     if (r0 >= (uint32_t)m0.x) return;
-    int const      first = (int)blockIdx.x, n = p.meta[2 * blockIdx.x + 1].x - first + 1;
+    int const      first = (int)blockIdx.x, n = m1.x - first + 1;
     uint32_t const rows = min((uint32_t)m0.x - r0, 16u), rr = threadIdx.x & 15, c4 = threadIdx.x >> 4;
     uint32_t const r = r0 + min(rr, rows - 1);
     auto  slot = [&](int i) { return (uint64_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * TR; };

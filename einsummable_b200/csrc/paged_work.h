@@ -453,10 +453,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     __shared__ float   so[WARPS][CHUNKS * 128];
     __shared__ float2  sml[WARPS];
     ES_PDL_PROLOGUE();
-    int4 const     m0 = p.meta[2 * blockIdx.x];
+    int4 const     m0 = p.meta[2 * blockIdx.x], m1 = p.meta[2 * blockIdx.x + 1]; // (m1 means something if m0.x > 0)
     uint32_t const r0 = blockIdx.y * 16;
     if (r0 >= (uint32_t)m0.x) return;
-    int const      first = (int)blockIdx.x, n = p.meta[2 * blockIdx.x + 1].x - first + 1;
+    int const      first = (int)blockIdx.x, n = m1.x - first + 1;
     uint32_t const rows = min((uint32_t)m0.x - r0, 16u), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t const at_once = min(rows, WARPS), slices = WARPS / at_once, slice = warp / at_once;
     for (uint32_t rr = 0; rr < rows; rr += at_once) {
@@ -467,7 +467,18 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
         float top = -INFINITY, l = 0.f, o[CHUNKS][4] = {};
         if (on) {
             for (int i0 = (int)slice * 32; i0 < n; i0 += (int)slices * 32) {
-                int const    i = i0 + (int)lane;
+                int const    i = i0 + (int)lane, here = min(32, n - i0);
+                float4       x[BATCH][CHUNKS];
+                auto         fetch = [&](int k0) { // (parts beyond the last: weight 0)
+#pragma unroll
+                    for (int k = 0; k < BATCH; ++k) {
+                        float const* src = p.part_out + slot(i0 + min(k0 + k, here - 1)) * p.part_d;
+#pragma unroll
+                        for (int c = 0; c < CHUNKS; ++c)
+                            if (c * 128 + lane * 4 < p.part_d) x[k][c] = *reinterpret_cast<float4 const*>(src + c * 128 + lane * 4);
+                    }
+                };
+                fetch(0);
                 float2 const ml = i < n ? p.part_ml[slot(i)] : make_float2(-INFINITY, 0.f);
                 float        tm = ml.y == 0.f ? -INFINITY : ml.x;
 #pragma unroll
@@ -486,28 +497,21 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 #pragma unroll
                 for (int x = 16; x; x >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
                 l += ls;
-                int const here = min(32, n - i0);
-                for (int k0 = 0; k0 < here; k0 += BATCH) { // (parts beyond the last: weight 0)
-                    float4 x[BATCH][CHUNKS];
-                    float  wk[BATCH];
+                for (int k0 = 0; k0 < here; k0 += BATCH) {
+                    if (k0) fetch(k0);
 #pragma unroll
                     for (int k = 0; k < BATCH; ++k) {
-                        float const* src = p.part_out + slot(i0 + min(k0 + k, here - 1)) * p.part_d;
-                        wk[k] = __shfl_sync(0xffffffffu, wgt, k0 + k);
+                        float const wk = __shfl_sync(0xffffffffu, wgt, k0 + k);
+                        if (k0 + k < here) {
 #pragma unroll
-                        for (int c = 0; c < CHUNKS; ++c)
-                            if (c * 128 + lane * 4 < p.part_d) x[k][c] = *reinterpret_cast<float4 const*>(src + c * 128 + lane * 4);
-                    }
-#pragma unroll
-                    for (int k = 0; k < BATCH; ++k)
-#pragma unroll
-                        for (int c = 0; c < CHUNKS; ++c)
-                            if (k0 + k < here) {
-                                o[c][0] = fmaf(x[k][c].x, wk[k], o[c][0]);
-                                o[c][1] = fmaf(x[k][c].y, wk[k], o[c][1]);
-                                o[c][2] = fmaf(x[k][c].z, wk[k], o[c][2]);
-                                o[c][3] = fmaf(x[k][c].w, wk[k], o[c][3]);
+                            for (int c = 0; c < CHUNKS; ++c) {
+                                o[c][0] = fmaf(x[k][c].x, wk, o[c][0]);
+                                o[c][1] = fmaf(x[k][c].y, wk, o[c][1]);
+                                o[c][2] = fmaf(x[k][c].z, wk, o[c][2]);
+                                o[c][3] = fmaf(x[k][c].w, wk, o[c][3]);
                             }
+                        }
+                    }
                 }
             }
         }
