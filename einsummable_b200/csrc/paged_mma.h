@@ -20,7 +20,7 @@
 namespace es {
 namespace {
 
-constexpr int MMA_BK = 16, MMA_OVH = 4, MMA_WARPS = 4, MMA_STAGES = 3;
+constexpr int MMA_BK = 16, MMA_OVH = 6, MMA_WARPS = 4, MMA_STAGES = 3;
 constexpr float MMA_RESCALE = 8.f;
 constexpr float MMA_NO_KEY = -1e30f; // the maximum before the first key: finite, so that no difference is inf - inf
 

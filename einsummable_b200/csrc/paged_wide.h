@@ -18,6 +18,8 @@
 //                    values.  (With every row's address sent through a shuffle a tile's 64 KB took 8700 cycles.)
 // TMEM: scores 2 x 128 columns, accumulators 2 x 128.  Products of one thread are done in order, so S_t of the
 // next tile may be issued over P_t as soon as P_t V is, and whoever sees S_t complete knows P_t V to be.
+// Tried and dropped: a third of the exponentials as polynomials on the fused multiply-add units (a 4096-token prompt
+// 171 -> 186 us), P handed over in halves (the same).
 // Every wait is bounded; on expiry the kernel records 0x31-0x39, lets its copies land, frees TMEM and returns.
 #pragma once
 #include "paged_mma.h"
@@ -276,25 +278,34 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
         // D = f32, A / B = f16, N >> 3, M >> 4; P V reads V with the head dim (its N) contiguous
         uint32_t const idesc_s = (1u << 4) | ((uint32_t)(BK >> 3) << 17) | ((128u >> 4) << 24);
         uint32_t const idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(DPAD >> 3) << 17) | ((128u >> 4) << 24);
+        // (every descriptor is formed by the whole warp, outside the one-lane region: formed inside it a product of
+        // K took 59 cycles to issue instead of 35)
         auto issue_s = [&](uint32_t t, uint32_t st) {
-            uint64_t const a = desc_hi | (uint64_t)((sQ + t * TILE) >> 4), b = desc_hi | (uint64_t)((sK + st * TILE) >> 4);
-            uint32_t const d = tmem + t * 128;
+            uint64_t const a0 = desc_hi | (uint64_t)((sQ + t * TILE) >> 4), b0 = desc_hi | (uint64_t)((sK + st * TILE) >> 4);
+            uint32_t const d = tmem + t * 128, bar = s_full + 8 * t;
+            uint64_t       a[KB * 4], b[KB * 4];
+#pragma unroll
+            for (uint32_t i = 0; i < KB * 4; ++i) {
+                uint64_t const o = (uint64_t)(((i >> 2) * BLOCK + (i & 3) * 32) >> 4);
+                a[i] = a0 + o;
+                b[i] = b0 + o;
+            }
             if (leader) {
 #pragma unroll
-                for (uint32_t i = 0; i < KB * 4; ++i) {
-                    uint64_t const o = (uint64_t)(((i >> 2) * BLOCK + (i & 3) * 32) >> 4);
-                    umma<0>(d, a + o, b + o, idesc_s, i ? 1u : 0u);
-                }
-                umma_commit(s_full + 8 * t);
+                for (uint32_t i = 0; i < KB * 4; ++i) umma<0>(d, a[i], b[i], idesc_s, i ? 1u : 0u);
+                umma_commit(bar);
             }
         };
         auto issue_o = [&](uint32_t t, uint32_t st, bool keep) {
-            uint64_t const b = desc_v | (uint64_t)((sV + st * TILE) >> 4);
-            uint32_t const d = tmem + 256 + t * 128, a = tmem + t * 128;
+            uint64_t const b0 = desc_v | (uint64_t)((sV + st * TILE) >> 4);
+            uint32_t const d = tmem + 256 + t * 128, a0 = tmem + t * 128;
+            uint64_t       b[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) b[i] = b0 + (uint64_t)((i * 2048) >> 4);
             if (leader) {
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) // 16 keys a product: 8 TMEM columns of P (over the scores of its 64 keys), 16 rows of V
-                    umma_ts(d, a + (i >> 2) * 64 + (i & 3) * 8, b + (uint64_t)((i * 2048) >> 4), idesc_o, (keep || i) ? 1u : 0u);
+                    umma_ts(d, a0 + (i >> 2) * 64 + (i & 3) * 8, b[i], idesc_o, (keep || i) ? 1u : 0u);
             }
         };
         auto commit = [&](uint32_t b) {
@@ -323,7 +334,10 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     uint32_t const at = tiles + j;
                     for (uint32_t t = 0; t < both; ++t) {
                         if (j == 0 && !(ok = wait(o_free + 8 * t, (n_o[t] & 1) ^ 1, 0x38))) break;
-                        if (t == 0 && !(ok = wait(v_full + 8 * (at & 1), (at >> 1) & 1, 0x33))) break;
+                        if (t == 0) { // this tile's values and the next one's keys, while the exponentials are under way
+                            if (!(ok = wait(v_full + 8 * (at & 1), (at >> 1) & 1, 0x33))) break;
+                            if (j + 1 < n_tiles && !(ok = wait(k_full + 8 * ((at + 1) & 1), ((at + 1) >> 1) & 1, 0x32))) break;
+                        }
                         if (!(ok = wait(p_ready + 8 * t, n_p[t] & 1, 0x34))) break;
                         ++n_p[t];
                         issue_o(t, at & 1, j != 0);
@@ -332,7 +346,6 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                             commit(o_done + 8 * t);
                             ++n_o[t];
                         } else {
-                            if (t == 0 && !(ok = wait(k_full + 8 * ((at + 1) & 1), ((at + 1) >> 1) & 1, 0x32))) break;
                             issue_s(t, (at + 1) & 1);
                             if (t + 1 == both) commit(k_empty + 8 * ((at + 1) & 1));
                         }
