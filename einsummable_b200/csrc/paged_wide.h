@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                         float v[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = f.wa == 0.f ? 0.f : __uint_as_float(x[i]) * f.wa; // a weight of 0: the sum may be anything
-                        if (f.wb != 0.f) {
+                        if (p.base_out && f.wb != 0.f) {
                             float const* base = p.base_out + at * p.d + e;
 #pragma unroll
                             for (int i = 0; i < 16; i += 4) {
@@ -657,7 +657,7 @@ template <int DPAD> __global__ void __launch_bounds__(256) paged_wide_join_kerne
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             v[k] = f.wa == 0.f ? 0.f : o[c][k] * f.wa;
-            if (f.wb != 0.f && e + k < p.d) v[k] = fmaf(p.base_out[at * p.d + e + k], f.wb, v[k]);
+            if (p.base_out && f.wb != 0.f && e + k < p.d) v[k] = fmaf(p.base_out[at * p.d + e + k], f.wb, v[k]);
         }
         *reinterpret_cast<float4*>(&so[rr][e]) = make_float4(v[0], v[1], v[2], v[3]);
     }

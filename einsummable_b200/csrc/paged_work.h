@@ -373,7 +373,8 @@ __device__ __forceinline__ void write_meta(paged_params_t const& p, work_t const
 
 // The weights that turn an unnormalised sum (reference point m in log2 units, sum of exponentials l) and,
 // where there is one, the prefix's normalised result (natural log lse) into the result:
-// out = wa * sum + wb * prefix.  No key at all: both weights 0, lse -inf.
+// out = wa * sum + wb * prefix.  No key at all: both weights 0, lse -inf.  Without a prefix wb is 0 whatever the
+// scores were: a weight that is not 0 is what lets the prefix's result be read.
 struct finish_t {
     float wa, wb, lse;
 };
@@ -392,7 +393,7 @@ __device__ __forceinline__ finish_t finish(float m, float l, bool has_base, floa
     float const b = b2 == -INFINITY ? 0.f : ex2(b2 - top);
     float const total = fmaf(l, a, b), inv = __fdividef(1.f, total);
     f.wa = a * inv;
-    f.wb = b * inv;
+    f.wb = has_base ? b * inv : 0.f; // (0 * inv may be NaN, and there is nothing to read)
     f.lse = (top + __log2f(total)) * LN_2;
     return f;
 }
