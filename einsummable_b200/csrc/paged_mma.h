@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                             s[nt][1][2 + x] = fmaf(s[nt][0][2 + x], p.scale_log2, -mn);
                         }
                 }
-                uint32_t b[NT][2];
+                uint32_t b[NT][2], low[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float e[4];
@@ -316,8 +316,15 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                     for (int i = 0; i < 4; ++i) e[i] = ex2(s[nt][1][i]);
                     l[nt][0] += e[0] + e[2]; // (the sum of the unrounded ones)
                     l[nt][1] += e[1] + e[3];
-                    b[nt][0] = transpose8x8(pack_h2(e[0], e[1]));
-                    b[nt][1] = transpose8x8(pack_h2(e[2], e[3]));
+                    // P as the sum of two f16: its rounding alone would cost as much as that of the result, and the matrix
+                    // units have time
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        uint32_t const hi = pack_h2(e[2 * x], e[2 * x + 1]);
+                        float2 const   f = __half22float2(*reinterpret_cast<__half2 const*>(&hi));
+                        b[nt][x] = transpose8x8(hi);
+                        low[nt][x] = transpose8x8(pack_h2(e[2 * x] - f.x, e[2 * x + 1] - f.y));
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < KS; ++i) {
@@ -325,7 +332,10 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                     if (i < 4) ldm4t<0>(st + vx[i & 3], a);
                     else ldm4t<128>(st + vx[i & 3], a);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][i], a, b[nt][0], b[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816(o[nt][i], a, b[nt][0], b[nt][1]);
+                        mma16816(o[nt][i], a, low[nt][0], low[nt][1]);
+                    }
                 }
                 st = st + stage_bytes == ring_end ? ring : st + stage_bytes;
             }
@@ -353,7 +363,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                             o[nt][i][x] *= f.wa;
                             o[nt][i][2 + x] *= f.wa;
                         }
-                        if (f.wb != 0.f) {
+                        if (p.base_out && f.wb != 0.f) {
                             float const* base = p.base_out + at * p.d + g;
 #pragma unroll
                             for (int i = 0; i < KS; ++i) {
