@@ -212,11 +212,12 @@ int es_b200_create(int device, es_b200_t** out)
             fail(ES_BAD_ARGUMENT, "device ordinal " + std::to_string(device) + " out of range");
         ES_CUDA_CHECK(cudaSetDevice(device));
         ES_CUDA_CHECK(cudaFree(nullptr));
-        cudaDeviceProp prop;
-        ES_CUDA_CHECK(cudaGetDeviceProperties(&prop, device));
-        if (prop.major != 10)
+        int major = 0, minor = 0; // (all of cudaDeviceProp takes a millisecond)
+        ES_CUDA_CHECK(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+        ES_CUDA_CHECK(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device));
+        if (major != 10)
             fail(ES_NOT_SUPPORTED, "es_b200 kernels are built for sm_100a only; device is sm_" +
-                                       std::to_string(prop.major) + std::to_string(prop.minor));
+                                       std::to_string(major) + std::to_string(minor));
         auto* h = new es_b200;
         h->device = device;
         for (auto& c : h->counters) c = 0;

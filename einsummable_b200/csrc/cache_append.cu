@@ -369,7 +369,7 @@ int launch_cache_append(es_cache_append_t const& a, es_cache_append_args_t const
     p.first_block[0] = (uint32_t)bq;
     p.first_block[1] = (uint32_t)(bq + bk);
     dim3 const  grid((uint32_t)(bq + 2 * bk));
-    pdl_scope_t scope(true); // (the kernel waits for those before it itself)
+    pdl_scope_t scope(pdl_allowed()); // (the kernel waits for those before it itself)
     auto        go = [&](auto kernel) { launch_k(kernel, grid, dim3(APPEND_THREADS), 0, stream, p); };
     auto        pick = [&](auto ti, auto tc) {
         using TI = decltype(ti);

@@ -270,7 +270,7 @@ void check_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
     if (!(a.scale >= 1e-30f && a.scale <= 1e30f)) fail(ES_BAD_DESCRIPTOR, "paged attention: the scale must lie in 1e-30 .. 1e30");
     if (!x.q || !x.k_cache || !x.v_cache || !x.out || !x.lengths || !x.tables) fail(ES_BAD_ARGUMENT, "paged attention: null pointer");
     if (!prefix && a.prefix_len) fail(ES_BAD_ARGUMENT, "paged attention: a prefix needs es_b200_launch_prefix_attention");
-    if (a.prefix_len > 0x7fffffffu) fail(ES_NOT_SUPPORTED, "paged attention: prefix beyond 31 bits");
+    if (a.prefix_len > MAX_TOKENS) fail(ES_NOT_SUPPORTED, "paged attention: prefix beyond 2^30 tokens");
     if (a.prefix_len && !x.prefix_pages) fail(ES_BAD_ARGUMENT, "paged attention: null list of the prefix's pages");
     if (!x.row_offsets && c.rows != c.batch) fail(ES_BAD_DESCRIPTOR, "paged attention: without row offsets there is one row a sequence");
     for (int i = 0; i != 2; ++i)
@@ -340,7 +340,7 @@ int launch_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
     uint64_t const all = (uint64_t)c.batch * a.prefix_len * c.kv_heads * c.head_dim * 2 * dtype_size(c.dtype);
     bool const     front = a.prefix_len && !x.row_offsets && p.group <= MMA_MAX_TR && all <= (64ull << 20);
     int            launches = 0;
-    pdl_scope_t    scope(true); // (every kernel waits for those before it itself)
+    pdl_scope_t    scope(pdl_allowed()); // (every kernel waits for those before it itself)
     if (front) {
         p.front = a.prefix_len;
         p.front_pages = x.prefix_pages;

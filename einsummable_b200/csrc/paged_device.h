@@ -40,11 +40,12 @@ __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ void  from_f32(float& y, float x) { y = x; }
 __device__ __forceinline__ void  from_f32(__half& y, float x) { y = __float2half_rn(x); }
 
-// tokens a sequence's row of pages can hold (lengths are 32-bit)
-inline uint32_t paged_capacity(es_paged_cache_t const& c)
+// Tokens a sequence's row of pages can hold; at most 2^30, so that a position and a few tiles fit 32 bits.
+constexpr uint32_t MAX_TOKENS = 1u << 30;
+inline uint32_t    paged_capacity(es_paged_cache_t const& c)
 {
     uint64_t const n = (uint64_t)c.table_stride * c.page_size;
-    return (uint32_t)(n < 0x7fffffffull ? n : 0x7fffffffull);
+    return (uint32_t)(n < MAX_TOKENS ? n : MAX_TOKENS);
 }
 
 inline void check_paged_cache(es_paged_cache_t const& c, char const* who)

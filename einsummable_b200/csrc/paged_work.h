@@ -323,8 +323,12 @@ template <int TR, int BK, int OVH> __device__ __forceinline__ void next_item(pag
         w.t = 0;
         if (++w.head == p.kv_heads) {
             w.head = 0;
-            do { // (ends: units are left, so a sequence with some follows)
-                w.s = get_sequence(p, ++w.seq);
+            do { // (units are left, so a sequence with some follows -- unless the arrays changed meanwhile)
+                if (++w.seq >= p.batch || p.prefix_len >= 0) {
+                    w.left = 0;
+                    return;
+                }
+                w.s = get_sequence(p, w.seq);
             } while (w.s.n == 0);
             w.rt = row_tiles<TR>(p, w.s);
         }

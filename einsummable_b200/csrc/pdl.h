@@ -10,6 +10,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <cstdlib>
 #include <utility>
 
 #include "common.h"
@@ -26,6 +27,16 @@ namespace es {
 // Set by the program executor around the launches of an op that may overlap the end of the op before it
 // on its lane; the launch helpers below then ask for programmatic stream serialization.
 bool& pdl_launch_flag();
+
+// ES_B200_PDL=0 in the environment: no programmatic dependent launch
+inline bool pdl_allowed()
+{
+    static bool const on = [] {
+        char const* v = std::getenv("ES_B200_PDL");
+        return !(v && v[0] == '0' && v[1] == 0);
+    }();
+    return on;
+}
 
 struct pdl_scope_t {
     bool saved;

@@ -277,7 +277,7 @@ int es_b200_launch_attention(es_b200_t* h, const es_attention_t* a, void* stream
  * dim contiguous.  What lies in the pages behind a sequence's last token is never used.
  *
  * What the arrays hold is checked on the device: a page number outside [0, n_pages) (0x21), a length
- * outside [0, table_stride * page_size] (0x22), row offsets that fall, go negative or pass `rows` (0x23), or
+ * outside [0, table_stride * page_size] or above 2^30 (0x22), row offsets that fall, go negative or pass `rows` (0x23), or
  * a position outside the table of angles (0x24) skips the access, leaves the rest of the batch right and
  * is reported by es_b200_device_status. */
 typedef struct {
@@ -330,13 +330,16 @@ int es_b200_launch_cache_append(es_b200_t* h, const es_cache_append_t* a, const 
  * A row that sees no key gets out = 0 and lse = -inf.  Query head h reads key / value head
  * h / (heads / kv_heads).  Any head dim up to 256, any strides; f16 with a head dim that is a multiple of
  * 8 up to 128, strides that are multiples of 8 and 16-byte aligned pointers runs on the tensor cores.
- * f32 accumulation and statistics; with f16 on the tensor cores the probabilities are rounded to f16 for
- * the product with the values.  Inside one sequence a masked token's values must be finite (0 * inf).
+ * f32 accumulation and statistics; where a key head serves more than 32 rows at once (parts of prompts, a
+ * batch behind a prefix) the probabilities are rounded to f16 for the product with the values.  A sequence
+ * without a key to see, NaN and infinities concern the rows that see them only -- and, on the tensor cores, the
+ * earlier rows of the same call in the same sequence, for which they are 0 times the value.
  * prefix_len tokens, the same for all sequences and listed by prefix_pages, can lie in front of every
  * sequence's own (es_b200_launch_prefix_attention): every row sees all of them, and they are read once
  * for the whole batch.  lengths and tables then count a sequence's own tokens only.
  * The workspace (es_b200_paged_attention_workspace; 16-byte aligned, contents irrelevant before and
- * after) may be shared by calls that do not overlap in time. */
+ * after) may be shared by calls that do not overlap in time.  out may not overlap q or the cache.  The same
+ * call gives the same bits.  Make one call on a device before capturing one. */
 typedef struct {
     es_paged_cache_t cache; /* dtype also of q and out */
     uint32_t heads;         /* a multiple of cache.kv_heads */

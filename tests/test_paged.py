@@ -65,7 +65,7 @@ def add_append(desc, **kw):
     (lambda: attention(scale=math.nan), _lib.ES_BAD_DESCRIPTOR),
     (lambda: attention(q_stride=(256, -64)), _lib.ES_BAD_DESCRIPTOR),
     (lambda: attention(prefix_len=10), _lib.ES_BAD_ARGUMENT),                 # and no list of its pages
-    (lambda: attention(prefix_len=1 << 31), _lib.ES_NOT_SUPPORTED),
+    (lambda: attention(prefix_len=(1 << 30) + 1), _lib.ES_NOT_SUPPORTED),
 ])
 def test_attention_refuses_descriptors(make, status):
     with pytest.raises(es.es_error) as e:
