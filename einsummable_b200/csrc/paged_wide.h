@@ -20,7 +20,7 @@
 // next tile may be issued over P_t as soon as P_t V is, and whoever sees S_t complete knows P_t V to be.
 // Tried and dropped: a third of the exponentials as polynomials on the fused multiply-add units (a 4096-token prompt
 // 171 -> 186 us), P handed over in halves (the same).
-// Every wait is bounded; on expiry the kernel records 0x31-0x39, lets its copies land, frees TMEM and returns.
+// Every wait is bounded; on expiry the kernel records 0x31-0x38, lets its copies land, frees TMEM and returns.
 #pragma once
 #include "paged_mma.h"
 
@@ -32,7 +32,7 @@ constexpr int      WIDE_TR = 256, WIDE_BK = 128, WIDE_OVH = 4, WIDE_SOFTMAX_WARP
 constexpr uint64_t WIDE_WAIT_LIMIT_CYCLES = 4000000000ull; // ~2 s at 2 GHz
 
 struct wide_ctrl_t {
-    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], o_free[2], pair[8];
+    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], o_free[2];
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
@@ -135,8 +135,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
     uint32_t const     bars = smem_u32(ctrl);
     // in the order of wide_ctrl_t
     uint32_t const     q_full = bars, k_full = q_full + 16, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16, s_full = v_empty + 16,
-                   p_ready = s_full + 16, o_done = p_ready + 16, o_free = o_done + 16,
-                   pair = o_free + 16;
+                   p_ready = s_full + 16, o_done = p_ready + 16, o_free = o_done + 16;
     int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -150,7 +149,6 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
             mbar_init(o_done + 8 * i, 1);
             mbar_init(o_free + 8 * i, 256);
         }
-        for (int i = 0; i < 8; ++i) mbar_init(pair + 8 * i, 64);
         ctrl->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -363,14 +361,19 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
         uint32_t const row_s = tmem + t * 128 + half * 64 + lanes, row_o = tmem + 256 + t * 128 + half * OH + lanes;
         uint32_t       n_s = 0, n_o = 0, turn = 0;
         bool           ok = true, split = false;
-        // x becomes the other thread's value (the two warps of a quarter meet)
-        auto exchange = [&](float& x) {
+        // The other thread's value.  The two warps of a quarter meet at a barrier without a limit: they go through the
+        // same items, tiles and decisions, also after a wait has given up (ok is false then, nothing is waited for any
+        // more and what is computed means nothing).
+        auto exchange = [&](float x) {
             row_value[turn][t][half][r_tile] = x;
-            mbar_arrive(pair + 8 * (t * 4 + quarter));
-            bool const met = __all_sync(0xffffffffu, wide_wait(p, pair + 8 * (t * 4 + quarter), turn, abort_flag, 0x39)) != 0;
-            x = row_value[turn][t][half ^ 1][r_tile];
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quarter) : "memory");
+            float const y = row_value[turn][t][half ^ 1][r_tile];
             turn ^= 1; // (a value is overwritten two meetings later)
-            return met;
+            return y;
+        };
+        auto wait = [&](uint32_t b, uint32_t parity, uint32_t code) {
+            if (ok) ok = __all_sync(0xffffffffu, wide_wait(p, b, parity, abort_flag, code)) != 0;
+            tc_fence_after();
         };
         // this warp's 16 query rows of an item's tile t (none if the item has no key tile here); tell_q follows
         auto load_q = [&](work_t const& x) -> bool {
@@ -397,7 +400,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
             mbar_arrive(q_full + 8 * t);
         };
         if (load_q(w)) tell_q();
-        while (w.left && ok) {
+        while (w.left) {
             uint32_t const n = min(w.kt - w.j, w.left), f0 = first_tile_of<OVH>(w.j), f1 = first_tile_of<OVH>(w.j + n);
             uint32_t const start = w.t * TR, count = min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
             uint32_t const r = t * 128 + r_tile;
@@ -414,38 +417,46 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                 uint32_t const pr = start + min(r, count - 1), tok = fdivide(pr, p.grp);
                 int const      vis = visible(p, w.s, (int)tok);
                 for (uint32_t j = f0; j < f1; ++j) {
-                    ok = __all_sync(0xffffffffu, wide_wait(p, s_full + 8 * t, n_s & 1, abort_flag, 0x35)) != 0;
-                    if (!ok) break;
+                    wait(s_full + 8 * t, n_s & 1, 0x35);
                     ++n_s;
-                    tc_fence_after();
                     // every product with this item's queries is done: the next item's may come
                     bool const more = j + 1 == f1 && load_next_q();
                     int const  allow = vis - (int)(j * BK + half * 64); // this row sees the first `allow` of the thread's keys
                     bool const mask = __any_sync(0xffffffffu, allow < 64);
-                    // The scores are read twice, 32 at a time (there are 96 registers): for the maximum, the second half
-                    // first, and for the exponentials, so that P of the first half may lie over scores that have been read.
-                    auto hide = [&](uint32_t (&v)[32], int first) {
+                    // The exponentials are taken against the maximum so far while this tile's is being found: once more
+                    // if it turns out to lie more than 2^8 above that (an item's first tile always; hardly ever another).
+                    // P stays in registers until then: it will lie over the scores.
+                    uint32_t y[32];
+                    uint64_t sum[2];
+#pragma unroll 1
+                    for (int attempt = 0; attempt < 2; ++attempt) {
+                        uint64_t const scale2 = pack2(p.scale_log2, p.scale_log2), m2 = pack2(-m, -m);
+                        float          mx[2] = {-INFINITY, -INFINITY};
+                        sum[0] = sum[1] = 0;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (first + i >= allow) v[i] = 0xff800000u; // -inf
-                    };
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    auto  largest = [&](uint32_t (&v)[32]) {
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t x[32];
+                            tmem_ld32(row_s + c * 32, x);
+                            if (mask) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-                    };
-                    uint32_t x[32];
-                    tmem_ld32(row_s + 32, x);
-                    if (mask) hide(x, 32);
-                    largest(x);
-                    tmem_ld32(row_s, x);
-                    if (mask) hide(x, 0);
-                    largest(x);
-                    float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-                    float others = top;
-                    if (!(ok = exchange(others))) break;
-                    top = fmaxf(top, others) * p.scale_log2;
-                    if (__any_sync(0xffffffffu, top > m + MMA_RESCALE)) { // (the same in both warps)
+                                for (int i = 0; i < 32; ++i)
+                                    if (c * 32 + i >= allow) x[i] = 0xff800000u; // -inf
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                float const s0 = __uint_as_float(x[2 * i]), s1 = __uint_as_float(x[2 * i + 1]);
+                                float       e0, e1;
+                                mx[i & 1] = max3(mx[i & 1], s0, s1);
+                                unpack2(fma2(pack2(s0, s1), scale2, m2), e0, e1);
+                                e0 = ex2(e0);
+                                e1 = ex2(e1);
+                                sum[i & 1] = add2(sum[i & 1], pack2(e0, e1));
+                                y[c * 16 + i] = pack_h2(e0, e1);
+                            }
+                        }
+                        float top = fmaxf(mx[0], mx[1]);
+                        top = fmaxf(top, exchange(top)) * p.scale_log2;
+                        if (!__any_sync(0xffffffffu, top > m + MMA_RESCALE)) break; // (the same in both warps)
                         float const mn = fmaxf(m, top), a = ex2(m - mn);
                         m = mn;
                         l *= a;
@@ -460,26 +471,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                             }
                         }
                     }
-                    uint64_t const scale2 = pack2(p.scale_log2, p.scale_log2), m2 = pack2(-m, -m);
-                    uint64_t       sum[2] = {0, 0};
-                    auto exponentials = [&](uint32_t (&v)[32], int c) { // of 32 scores, into P's columns 16 c ..
-                        uint32_t y[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            float e0, e1;
-                            unpack2(fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, m2), e0, e1);
-                            e0 = ex2(e0);
-                            e1 = ex2(e1);
-                            sum[i & 1] = add2(sum[i & 1], pack2(e0, e1));
-                            y[i] = pack_h2(e0, e1);
-                        }
-                        tmem_st16(row_s + c * 16, y);
-                    };
-                    exponentials(x, 0);
-                    tmem_ld32(row_s + 32, x);
-                    if (mask) hide(x, 32);
-                    exponentials(x, 1);
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tmem_st32(row_s, y); // (waits for the stores to be done)
                     tc_fence_before();
                     mbar_arrive(p_ready + 8 * t);
                     float s0, s1;
@@ -487,15 +479,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     l += s0 + s1;
                     if (more) tell_q();
                 }
-                if (!ok) break;
-                float others = l;
-                if (!(ok = exchange(others))) break;
+                float const others = exchange(l);
                 l = half ? others + l : l + others; // (the same sum in both)
                 if (f1 > f0) {
-                    ok = __all_sync(0xffffffffu, wide_wait(p, o_done + 8 * t, n_o & 1, abort_flag, 0x36)) != 0;
-                    if (!ok) break;
+                    wait(o_done + 8 * t, n_o & 1, 0x36);
                     ++n_o;
-                    tc_fence_after();
                 }
                 int const      row = w.s.row0 + (int)tok;
                 uint32_t const head = w.head * p.group + (pr - tok * p.group);

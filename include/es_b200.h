@@ -411,7 +411,7 @@ int es_b200_rowsum_f32_noalloc(es_b200_t*   h,
  * tensor-core kernels: 0 = fine; nonzero = a bounded wait inside a kernel gave
  * up (1 producer, 2/3 MMA issuer, 4 epilogue) and that launch's output is not
  * valid; 0x11..0x16 = the same inside the attention kernel (Q copy, K copy, scores, P tile,
- * V copy, P V), 0x21..0x24 = what a paged-cache kernel found in its arrays, 0x31..0x39 = a wait inside
+ * V copy, P V), 0x21..0x24 = what a paged-cache kernel found in its arrays, 0x31..0x38 = a wait inside
  * the paged attention kernel.  The reference has no counterpart: its library kernels cannot report. */
 int es_b200_device_status(es_b200_t* h, unsigned int* error_word);
 
