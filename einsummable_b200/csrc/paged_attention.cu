@@ -23,7 +23,7 @@ namespace {
 __device__ unsigned int g_paged_error;
 
 constexpr uint32_t SIMT_BLOCKS = 2 * SM_COUNT;
-constexpr uint32_t MMA_BLOCKS = 2 * SM_COUNT, MMA_WORKERS = MMA_BLOCKS * MMA_WARPS, MMA_MAX_TR = 32;
+constexpr uint32_t MMA_BLOCKS = 2 * SM_COUNT, MMA_WORKERS = MMA_BLOCKS * MMA_WARPS, MMA_MAX_TR = 16;
 constexpr uint32_t WIDE_BLOCKS = SM_COUNT;
 
 uint64_t align256(uint64_t x)
@@ -140,7 +140,7 @@ template <typename T, bool VEC> part_t simt_part(paged_params_t const& p)
     if (p.d <= 64) {
         if constexpr (sizeof(T) == 4) {
             if (one) return simt_as<T, 2, 1, VEC>(p);
-            if (p.group > 4) return simt_as<T, 2, 8, VEC>(p);
+            if (p.group > 4 || p.prefix_len >= 0) return simt_as<T, 2, 8, VEC>(p);
         }
         return simt_as<T, 2, 4, VEC>(p);
     }
@@ -248,7 +248,8 @@ int choose(paged_params_t const& q, int dtype, bool vec, part_t (&c)[2])
     if (fewest <= MMA_MAX_TR) {
         p.packed_max = MMA_MAX_TR;
         uint32_t const rows = p.prefix_len >= 0 ? most : p.group; // of an item, where tokens come singly
-        c[n++] = rows <= 8 ? mma_part<1>(p) : rows <= 16 ? mma_part<2>(p) : mma_part<4>(p);
+        // (tiles of 32 rows spill: 8 sequences of 4 query heads a key head behind 8000 tokens took 76 us, 41 with tcgen05)
+        c[n++] = rows <= 8 ? mma_part<1>(p) : mma_part<2>(p);
     }
     if (most > MMA_MAX_TR) {
         p.packed_min = MMA_MAX_TR;
@@ -333,12 +334,16 @@ int launch_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
     p.scale_log2 = a.scale * LOG2_E;
     p.error = error_address();
     bool const vec = aligned16(a, x);
-    // A short prefix is read by every sequence for itself, in front of its own keys and out of the L2 cache:
-    // with up to 64 MB read in all that takes less than the two kernels that reading it once would add (3
-    // sequences behind 500 tokens: 25 us shared, 11 us so).  Single tokens only: parts of prompts have rows
-    // enough to share.
+    // A short prefix is read by every sequence for itself, in front of its own keys and out of the L2 cache: one
+    // kernel and a join.  Reading it once adds two kernels -- few rows: the same kind again (8 sequences of 32 key
+    // heads behind 1000 tokens, 131 MB read in all: 25 us shared, 29 in front; 65 MB: equal), more: tcgen05's, whose
+    // start alone is worth some 20 us (16 sequences of 8 key heads behind 1000 / 2000 / 4000 tokens, 65 / 131 / 262
+    // MB: 37 / 37 / 37 us shared, 22 / 29 / 39 in front).  Single tokens only: parts of prompts have rows enough to
+    // share.
+    bool const     tc = c.dtype == ES_F16 && vec && c.head_dim <= 128;
     uint64_t const all = (uint64_t)c.batch * a.prefix_len * c.kv_heads * c.head_dim * 2 * dtype_size(c.dtype);
-    bool const     front = a.prefix_len && !x.row_offsets && p.group <= MMA_MAX_TR && all <= (64ull << 20);
+    uint64_t const most = (tc && c.rows * p.group > MMA_MAX_TR ? 224ull : 64ull) << 20;
+    bool const     front = a.prefix_len && !x.row_offsets && (!tc || p.group <= MMA_MAX_TR) && all <= most;
     int            launches = 0;
     pdl_scope_t    scope(pdl_allowed()); // (every kernel waits for those before it itself)
     if (front) {

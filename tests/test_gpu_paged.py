@@ -59,6 +59,8 @@ ATTENTION = [
     ([1] * 9, [0, 1, 14, 15, 16, 62, 126, 127, 700], 8, 8, 80, 7, {}),  # pages that end inside a tile
     ([1] * 3, [511, 512, 2000], 28, 4, 112, 48, {}),                 # 7 query heads a key head
     ([1], [900], 40, 1, 128, 32, {}),                                # 40 query heads on one key head
+    ([1, 1], [1900, 20], 32, 2, 128, 16, {}),                        # 16
+    ([1, 1], [1900, 20], 34, 2, 64, 16, {}),                         # 17
     ([1, 1], [300, 40], 64, 1, 96, 1, {}),                           # pages of one token
     ([1] * 300, [(37 * i) % 90 - 1 for i in range(300)], 4, 2, 32, 16, {}),  # more sequences than threads of a block
     ([1, 1], [700, 90], 12, 4, 128, 16, {"layout": "head"}),
@@ -111,6 +113,9 @@ PREFIX = [
     ([1] * 4, [5, 0, 70, 260], 8, 4, 64, 16, 15, {}),               # a prefix that ends inside a key tile
     ([1] * 9, [5, 0, 70, 260, 1, 2, 3, 4, 5], 8, 4, 64, 24, 100, {}),
     ([1] * 40, [i for i in range(40)], 32, 1, 128, 16, 200, {"offsets": True}),  # 32 heads on one key head: 1280 rows
+    ([1] * 70, [i % 33 for i in range(70)], 8, 2, 128, 16, 4000, {}),            # read once, 280 rows a key head
+    ([1] * 4, [3, 0, 17, -1], 8, 2, 128, 16, 3500, {"offsets": True}),           # 16 rows
+    ([1] * 5, [3, 0, 17, -1, 40], 8, 2, 64, 24, 900, {"offsets": True}),         # 20
 ]
 
 
