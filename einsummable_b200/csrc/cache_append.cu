@@ -9,7 +9,9 @@
 // thread, for several rows: what a row needs to know first is a chain of loads -- its sequence (found by counting, a
 // lane a sequence, how many end at or before the row), the sequence's length, the page -- and a block's warps find
 // the places of all its rows before it moves them.  Moves are short chains of loads, so warps count: 40 an SM.  The
-// blocks make one wave.
+// blocks make one wave.  Measured: 7311 rows of 32 + 64 heads of 128, f16 (361 MB) 70 us = 5.1 TB/s (a row a block, its
+// places found by every block for itself: 75 us; six heads of a thread at once: 97, with half the warps); a row of
+// one sequence 3 us.
 #include <cuda_fp16.h>
 
 #include <algorithm>

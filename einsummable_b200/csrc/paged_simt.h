@@ -6,8 +6,9 @@
 // exchanged between groups until the segment ends.  The query rows stay in registers, multiplied by
 // scale * log2 e.  The next KEYS keys and values are loaded before the current ones are used.  Bound: the latency
 // of those loads for short sequences, memory for long ones with up to TR packed rows a key head; beyond that a key
-// is read once per TR rows.  TR follows the rows there are (12 sequences of up to 2900 tokens, 4 query heads of 64
-// a key head: 17 us with 8 rows and one key at a time).
+// is read once per TR rows, and the multiply-adds with their shuffles are what it waits for.  TR follows the rows
+// there are: 12 sequences of up to 2900 tokens, 4 query heads of 64 a key head, 14.5 MB: 17 us with 8 rows and one
+// key at a time, 13 with 4 rows and two keys, 15.6 with the join -- launch, counting and the first loads are most of it.
 #pragma once
 #include "paged_work.h"
 

@@ -2,14 +2,16 @@
 // the fifth-generation tensor cores.
 //
 // Bound: the tensor cores, and as much the exponentials: a tile of 128 rows x 128 keys of 128 elements is 2 * 512
-// cycles of products and, at 16 exponentials a cycle, 1024 of softmax.  So an item is two tiles of 128 packed rows
+// cycles of products and, at 16 exponentials a cycle, 1024 of softmax.  (Measured: 1330 and 1940 with what lies between
+// them, 3500 for the pair of tiles; 256 rows a key head behind 16000 shared tokens 16.9 GF in 30 us, a prompt of 4096
+// tokens with 32 heads 137 GF in 168 us = 0.82 PFLOP/s, where the first tile of a block alone takes 5 us.)  So an item is two tiles of 128 packed rows
 // that share the keys in shared memory and take turns: while one tile's scores are on the tensor cores, the
 // other's are exponentials.  One persistent block an SM, 20 warps:
-//   warps 0-7, 8-15  softmax of tile 0 / 1, two threads a row (= TMEM lane), 64 keys each -- with one thread a row the
-//                    chain scores, maximum, 128 exponentials, products took 3500 cycles a tile: maximum of the
-//                    scores, rescaling of the accumulator when it has moved by more than 2^8, exponentials (f32;
-//                    rounded to f16 for the product with the values), written as f16 pairs over the scores they
-//                    came from; and the copies of the tile's queries, those of the next item as soon as the last
+//   warps 0-7, 8-15  softmax of tile 0 / 1, two threads a row (= TMEM lane), 64 keys each -- half the
+//                    chain of one thread a row, and half the time results take to leave: exponentials (f32; rounded to
+//                    f16 for the product with the values) against the maximum so far, the maximum of the scores in the
+//                    same pass, both once more and the accumulator rescaled when it has moved by more than 2^8; written
+//                    as f16 pairs over the scores they came from; and the copies of the tile's queries, those of the next item as soon as the last
 //                    scores are there
 //   warp 16          issues the products: S_t = Q_t K^T into TMEM, O_t += P_t V with P_t read from TMEM
 //   warps 17-19      copy the pages into the 128-byte-swizzled tiles the tensor cores read, 16 keys of one page at a
@@ -19,7 +21,8 @@
 // TMEM: scores 2 x 128 columns, accumulators 2 x 128.  Products of one thread are done in order, so S_t of the
 // next tile may be issued over P_t as soon as P_t V is, and whoever sees S_t complete knows P_t V to be.
 // Tried and dropped: a third of the exponentials as polynomials on the fused multiply-add units (a 4096-token prompt
-// 171 -> 186 us), P handed over in halves (the same).
+// 171 -> 186 us), P handed over in halves (the same), a first pass over an empty tile to warm the instruction cache
+// (64 sequences behind 16000 tokens 60 -> 66 us).
 // Every wait is bounded; on expiry the kernel records 0x31-0x38, lets its copies land, frees TMEM and returns.
 #pragma once
 #include "paged_mma.h"
