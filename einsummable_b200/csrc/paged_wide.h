@@ -23,7 +23,7 @@
 // Tried and dropped: a third of the exponentials as polynomials on the fused multiply-add units (a 4096-token prompt
 // 171 -> 186 us), P handed over in halves (the same), a first pass over an empty tile to warm the instruction cache
 // (64 sequences behind 16000 tokens 60 -> 66 us).
-// Every wait is bounded; on expiry the kernel records 0x31-0x38, lets its copies land, frees TMEM and returns.
+// Every wait is bounded; on expiry the kernel records 0x31-0x39, lets its copies land, frees TMEM and returns.
 #pragma once
 #include "paged_mma.h"
 
@@ -35,7 +35,7 @@ constexpr int      WIDE_TR = 256, WIDE_BK = 128, WIDE_OVH = 4, WIDE_SOFTMAX_WARP
 constexpr uint64_t WIDE_WAIT_LIMIT_CYCLES = 4000000000ull; // ~2 s at 2 GHz
 
 struct wide_ctrl_t {
-    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], o_free[2];
+    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], o_free[2], pair[8];
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
@@ -138,7 +138,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
     uint32_t const     bars = smem_u32(ctrl);
     // in the order of wide_ctrl_t
     uint32_t const     q_full = bars, k_full = q_full + 16, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16, s_full = v_empty + 16,
-                   p_ready = s_full + 16, o_done = p_ready + 16, o_free = o_done + 16;
+                   p_ready = s_full + 16, o_done = p_ready + 16, o_free = o_done + 16,
+                   pair = o_free + 16;
     int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -152,6 +153,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
             mbar_init(o_done + 8 * i, 1);
             mbar_init(o_free + 8 * i, 256);
         }
+        for (int i = 0; i < 8; ++i) mbar_init(pair + 8 * i, 64);
         ctrl->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -364,19 +366,20 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
         uint32_t const row_s = tmem + t * 128 + half * 64 + lanes, row_o = tmem + 256 + t * 128 + half * OH + lanes;
         uint32_t       n_s = 0, n_o = 0, turn = 0;
         bool           ok = true, split = false;
-        // The other thread's value.  The two warps of a quarter meet at a barrier without a limit: they go through the
-        // same items, tiles and decisions, also after a wait has given up (ok is false then, nothing is waited for any
-        // more and what is computed means nothing).
-        auto exchange = [&](float x) {
-            row_value[turn][t][half][r_tile] = x;
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quarter) : "memory");
-            float const y = row_value[turn][t][half ^ 1][r_tile];
-            turn ^= 1; // (a value is overwritten two meetings later)
-            return y;
-        };
+        // (after a wait has given up nothing is waited for any more, and what is computed means nothing)
         auto wait = [&](uint32_t b, uint32_t parity, uint32_t code) {
             if (ok) ok = __all_sync(0xffffffffu, wide_wait(p, b, parity, abort_flag, code)) != 0;
             tc_fence_after();
+        };
+        // the other thread's value (the two warps of a quarter meet)
+        auto exchange = [&](float x) {
+            uint32_t const meet = pair + 8 * (t * 4 + quarter);
+            row_value[turn][t][half][r_tile] = x;
+            mbar_arrive(meet);
+            wait(meet, turn, 0x39);
+            float const y = row_value[turn][t][half ^ 1][r_tile];
+            turn ^= 1; // (a value is overwritten two meetings later)
+            return y;
         };
         // this warp's 16 query rows of an item's tile t (none if the item has no key tile here); tell_q follows
         auto load_q = [&](work_t const& x) -> bool {

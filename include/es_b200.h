@@ -264,7 +264,7 @@ int es_b200_launch_attention(es_b200_t* h, const es_attention_t* a, void* stream
  * list of pages (a row of `tables`) and a length, and may grow without anything being moved.
  *
  * The batch of one step, given to every call of the step (arrays in device memory, read when the kernels
- * run, so that a captured step can be replayed after they changed):
+ * run, so that a captured step can be replayed after they changed; not to be written while they run):
  *   lengths[batch]             tokens of the sequence in the cache, the new ones of this step included
  *   tables[batch][table_stride] pages of the sequence, in order; entries behind its last page are not read
  *   row_offsets[batch + 1]     row r of the step's tensors belongs to sequence i when row_offsets[i] <= r <
@@ -411,7 +411,7 @@ int es_b200_rowsum_f32_noalloc(es_b200_t*   h,
  * tensor-core kernels: 0 = fine; nonzero = a bounded wait inside a kernel gave
  * up (1 producer, 2/3 MMA issuer, 4 epilogue) and that launch's output is not
  * valid; 0x11..0x16 = the same inside the attention kernel (Q copy, K copy, scores, P tile,
- * V copy, P V), 0x21..0x24 = what a paged-cache kernel found in its arrays, 0x31..0x38 = a wait inside
+ * V copy, P V), 0x21..0x24 = what a paged-cache kernel found in its arrays, 0x31..0x39 = a wait inside
  * the paged attention kernel.  The reference has no counterpart: its library kernels cannot report. */
 int es_b200_device_status(es_b200_t* h, unsigned int* error_word);
 
