@@ -173,15 +173,25 @@ template <int DPAD, int NT, bool PAGE16> part_t mma_as(paged_params_t p)
     constexpr uint32_t TR = 8 * NT;
     part_t             c;
     p.part_d = DPAD;
-    // Direct: with at most 16 key tiles an item, one warp an item and no join
-    p.direct = !p.row_offsets && p.prefix_len < 0 && most_keys(p) <= 16 * MMA_BK && p.batch <= 65535;
+    // Direct: nothing is counted, and there is no join kernel.  While no block takes a second item: a block each, if a
+    // warp's part is at most 16 tiles (32 heads on 8, cut / a block each: 1 x 500 keys 17.3 / 14.3 us, 4 x 500 19.4 /
+    // 14.3, 36 x 1000 46 / 39, and 1 x 1000 19.4 / 19.5); more of them: a warp each, if its 16 tiles are the whole item
+    // (1 x 250 keys 19.5 us that way, 11.2 a block each; 16 x 250 20.4 and 13.2).
+    uint32_t const items = p.kv_heads * ((p.group + TR - 1) / TR); // of a sequence
+    uint64_t const all = (uint64_t)p.batch * items, keys = most_keys(p);
+    p.direct = DIRECT_NO;
+    if (!p.row_offsets && p.prefix_len < 0 && p.batch <= 65535) {
+        if (all <= MMA_BLOCKS && keys <= 16 * MMA_BK * MMA_WARPS) p.direct = DIRECT_BLOCK;
+        else if (keys <= 16 * MMA_BK) p.direct = DIRECT_WORKER;
+    }
     p.min_units = 4;
     c.p = p;
     c.main = [](paged_params_t const& p, cudaStream_t s) {
         static bool done[64] = {};
         allow_smem(paged_mma_kernel<DPAD, NT, PAGE16>, MMA_WARPS * mma_warp_bytes<DPAD>(TR), done);
         uint32_t const items = p.kv_heads * ((p.group + TR - 1) / TR); // of a sequence
-        dim3 const     grid(p.direct ? (items + MMA_WARPS - 1) / MMA_WARPS : MMA_BLOCKS, p.direct ? p.batch : 1);
+        dim3 const     grid(p.direct == DIRECT_BLOCK ? items : p.direct ? (items + MMA_WARPS - 1) / MMA_WARPS : MMA_BLOCKS,
+                            p.direct ? p.batch : 1);
         // rows of a query tile: the packed rows of one token, or of all there are
         uint32_t const q_rows = std::min(uint32_t(TR), !p.row_offsets && p.prefix_len < 0 ? p.group : p.rows * p.group);
         launch_k(paged_mma_kernel<DPAD, NT, PAGE16>, grid, dim3(MMA_WARPS * 32), MMA_WARPS * mma_warp_bytes<DPAD>(q_rows), s, p, q_rows);

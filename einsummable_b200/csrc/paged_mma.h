@@ -342,6 +342,28 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                 }
                 st = st + stage_bytes == ring_end ? ring : st + stage_bytes;
             }
+            if (p.direct == DIRECT_BLOCK) { // into this warp's ring, which is done with: maxima and sums, then the rows
+                __syncwarp();
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], d);
+                        uint32_t const r = nt * 8 + t4 * 2 + x;
+                        float* const   mine = reinterpret_cast<float*>(smem_mma + warp * MMA_STAGES * stage_bytes);
+                        if (g == 0) {
+                            mine[2 * r] = m[nt][x];
+                            mine[2 * r + 1] = l[nt][x];
+                        }
+#pragma unroll
+                        for (int i = 0; i < KS; ++i) {
+                            mine[2 * TR + r * DPAD + i * 16 + g] = o[nt][i][x];
+                            mine[2 * TR + r * DPAD + i * 16 + g + 8] = o[nt][i][2 + x];
+                        }
+                    }
+                break;
+            }
             int const to = segment_slot(w, n_units);
             if (to < 0 && p.base_out) wait_for_base(p);
 #pragma unroll
@@ -412,6 +434,41 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
             next_item<TR, BK, OVH>(p, w, n_units);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    if (p.direct == DIRECT_BLOCK && w.s.n > 0) { // (the same in the whole block)
+        if (w.left == 0 && lane < TR) { // no tile for this warp: nothing to add (its rows stay unread)
+            float* const mine = reinterpret_cast<float*>(smem_mma + warp * MMA_STAGES * stage_bytes);
+            mine[2 * lane] = MMA_NO_KEY;
+            mine[2 * lane + 1] = 0.f;
+        }
+        if (p.base_out) wait_for_base(p);
+        __syncthreads();
+        uint32_t const start = w.t * TR, count = min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
+        for (uint32_t i = threadIdx.x; i < count * (DPAD / 2); i += THREADS) { // two elements of a row
+            uint32_t const r = i / (DPAD / 2), e = i % (DPAD / 2) * 2;
+            auto           of = [&](int x) { return reinterpret_cast<float const*>(smem_mma + x * MMA_STAGES * stage_bytes); };
+            float          top = -INFINITY, l = 0.f, v[2] = {0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < MMA_WARPS; ++x)
+                if (of(x)[2 * r + 1] != 0.f) top = fmaxf(top, of(x)[2 * r]);
+#pragma unroll
+            for (int x = 0; x < MMA_WARPS; ++x) {
+                float const lx = of(x)[2 * r + 1];
+                if (lx == 0.f) continue;
+                float const  wgt = ex2(of(x)[2 * r] - (top == -INFINITY ? 0.f : top));
+                float2 const y = *reinterpret_cast<float2 const*>(of(x) + 2 * TR + r * DPAD + e);
+                l = fmaf(lx, wgt, l);
+                v[0] = fmaf(y.x, wgt, v[0]);
+                v[1] = fmaf(y.y, wgt, v[1]);
+            }
+            uint32_t const pr = start + r, tok = fdivide(pr, p.grp);
+            int const      row = w.s.row0 + (int)tok;
+            uint32_t const head = w.head * p.group + (pr - tok * p.group);
+            uint64_t const at = (uint64_t)row * p.heads + head;
+            finish_t const f = finish(top, l, p.base_lse != nullptr, p.base_lse ? p.base_lse[at] : 0.f);
+            if (e < p.d) write_out<__half, 2>(p, row, head, e, v, f, true);
+            if (e == 0 && p.lse) p.lse[at] = f.lse;
+        }
     }
     if (!split && !p.direct && lane == 0) write_meta<TR>(p, w, false);
     wait_for_base(p);

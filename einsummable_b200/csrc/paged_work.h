@@ -49,7 +49,7 @@ struct paged_params_t {
     int32_t        prefix_len;  // >= 0: all rows attend the one list of pages `tables`, of this many tokens
     int32_t const* front_pages; // front > 0: so many tokens, listed here, lie in front of every sequence's own (each
     uint32_t       front;       // sequence reads them for itself); their last key tile is not shared with its own
-    int32_t        direct;      // one worker an item: nothing is split (one row a sequence)
+    int32_t        direct;      // nothing is split among workers (one row a sequence): DIRECT_*
     uint32_t       packed_min, packed_max; // sequences with more than / at most so many packed rows
     uint32_t       min_units;   // a worker's share is at least this
     float          scale_log2;  // scale * log2 e
@@ -57,6 +57,10 @@ struct paged_params_t {
     int32_t        order;       // ORDER_*: when the kernel waits for the kernels before it
     unsigned int*  error;
 };
+
+// DIRECT_WORKER: one worker an item.  DIRECT_BLOCK: the warps of a block share an item's key tiles out among
+// themselves and join what they have in shared memory.
+enum { DIRECT_NO = 0, DIRECT_WORKER = 1, DIRECT_BLOCK = 2 };
 
 // Programmatic dependent launch between the kernels of one call (pdl.h).  A kernel starts when the one before it
 // has let it; what it may touch then is another matter:
@@ -203,18 +207,25 @@ __device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sc
     if (p.direct) {
         // one row a sequence: blocks (items of a sequence, sequences); nothing to count
         w.rt = (p.group + TR - 1) / TR;
-        w.head = w.worker;
+        w.head = p.direct == DIRECT_BLOCK ? blockIdx.x : w.worker;
         w.t = 0;
         if (w.rt > 1) {
-            w.head = w.worker / w.rt;
-            w.t = w.worker - w.head * w.rt;
+            uint32_t const item = w.head;
+            w.head = item / w.rt;
+            w.t = item - w.head * w.rt;
         }
         w.seq = blockIdx.y;
+        w.s.n = 0;
         if (w.head >= p.kv_heads) return;
         w.s = get_sequence(p, w.seq);
         if (w.s.n == 0) return;
         w.kt = tile_units<TR, BK, OVH>(p, w.s, w.t);
         w.left = w.kt;
+        if (p.direct == DIRECT_BLOCK) { // this warp's part of the tiles
+            uint32_t const tiles = w.kt - OVH, from = tiles * warp / (NT / 32);
+            w.j = OVH + from;
+            w.left = tiles * (warp + 1) / (NT / 32) - from;
+        }
         return;
     }
     uint64_t   mine = 0, u0 = 0;

@@ -89,6 +89,19 @@ def test_paged_attention(km, new, past, heads, kv_heads, dim, page, opt):
     run_and_check(km, batch_t(new, past, heads, kv_heads, dim, page, seed=len(new) + dim, **opt))
 
 
+@pytest.mark.parametrize("past,heads,kv_heads,dim,page,prefix", [
+    # no tile, one, as many as the block has warps, one more, ... up to the longest that a block takes
+    ([-1, 0, 15, 16, 46, 47, 63, 64, 65, 1023], 32, 8, 128, 16, 0),
+    ([-1, 0, 15, 16, 46, 47, 63, 64, 65, 700], 14, 2, 80, 7, 0),
+    ([1023, 5], 16, 1, 64, 64, 0),
+    ([300, 0, -1], 80, 2, 128, 16, 0),
+    ([300, 0, -1], 16, 4, 128, 16, 37),                          # a prefix in front of each
+    ([17, 0, -1, 500], 16, 4, 64, 16, 40000),                    # one that is joined in
+])
+def test_a_block_a_sequence_and_key_head(km, past, heads, kv_heads, dim, page, prefix):
+    run_and_check(km, batch_t([1] * len(past), past, heads, kv_heads, dim, page, prefix=prefix, seed=dim + prefix))
+
+
 @pytest.mark.parametrize("new,past", [([1, 1, 1], [7, 400, -1]), ([3, 70], [150, 12])])
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_not_causal(km, new, past, dtype):
