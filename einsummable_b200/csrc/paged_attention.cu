@@ -187,14 +187,15 @@ template <int DPAD, int NT, bool PAGE16> part_t mma_as(paged_params_t p)
     p.min_units = 4;
     c.p = p;
     c.main = [](paged_params_t const& p, cudaStream_t s) {
-        static bool done[64] = {};
-        allow_smem(paged_mma_kernel<DPAD, NT, PAGE16>, MMA_WARPS * mma_warp_bytes<DPAD>(TR), done);
+        static bool done[2][64] = {};
+        auto* const kernel = p.base_out ? paged_mma_kernel<DPAD, NT, PAGE16, true> : paged_mma_kernel<DPAD, NT, PAGE16, false>;
+        allow_smem(kernel, MMA_WARPS * mma_warp_bytes<DPAD>(TR), done[p.base_out ? 1 : 0]);
         uint32_t const items = p.kv_heads * ((p.group + TR - 1) / TR); // of a sequence
         dim3 const     grid(p.direct == DIRECT_BLOCK ? items : p.direct ? (items + MMA_WARPS - 1) / MMA_WARPS : MMA_BLOCKS,
                             p.direct ? p.batch : 1);
         // rows of a query tile: the packed rows of one token, or of all there are
         uint32_t const q_rows = std::min(uint32_t(TR), !p.row_offsets && p.prefix_len < 0 ? p.group : p.rows * p.group);
-        launch_k(paged_mma_kernel<DPAD, NT, PAGE16>, grid, dim3(MMA_WARPS * 32), MMA_WARPS * mma_warp_bytes<DPAD>(q_rows), s, p, q_rows);
+        launch_k(kernel, grid, dim3(MMA_WARPS * 32), MMA_WARPS * mma_warp_bytes<DPAD>(q_rows), s, p, q_rows);
     };
     c.join = nullptr;
     if (!p.direct)

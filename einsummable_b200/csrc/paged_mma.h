@@ -77,8 +77,9 @@ template <int DPAD> constexpr uint32_t mma_warp_bytes(uint32_t q_rows)
     return MMA_STAGES * (2 * MMA_BK * DPAD * 2 + q_rows * DPAD * 2);
 }
 
-// NT: tiles of 8 packed rows an item; PAGE16: pages are a multiple of 16 tokens, so that a tile lies in one
-template <int DPAD, int NT, bool PAGE16>
+// NT: tiles of 8 packed rows an item; PAGE16: pages are a multiple of 16 tokens, so that a tile lies in one; BASE: a
+// prefix's result is merged in (a kernel of its own, for the registers that takes)
+template <int DPAD, int NT, bool PAGE16, bool BASE>
 __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __grid_constant__ paged_params_t p, uint32_t q_rows)
 {
     constexpr int TR = 8 * NT, BK = MMA_BK, OVH = MMA_OVH, THREADS = MMA_WARPS * 32, CH = DPAD / 8; // CH: 16-byte chunks a row
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                 break;
             }
             int const to = segment_slot(w, n_units);
-            if (to < 0 && p.base_out) wait_for_base(p);
+            if (BASE && to < 0) wait_for_base(p);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -377,7 +378,16 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                     if (to < 0) {
                         uint32_t const pr = start + r, tok = fdivide(pr, p.grp);
                         uint64_t const at = (uint64_t)(w.s.row0 + (int)tok) * p.heads + w.head * p.group + (pr - tok * p.group);
-                        finish_t const f = finish(m[nt][x], l[nt][x], p.base_lse != nullptr, p.base_lse ? p.base_lse[at] : 0.f);
+                        // the prefix's row comes beside its weight, not behind it (250 sequences x 32 heads, 8000 items of 4 tiles:
+                        // 71 -> 65 us; fetched a tile earlier: 66, and a batch of 64 then took 19 instead of 15); with 16 rows a
+                        // tile there is no room for it
+                        float bases[2 * KS];
+                        if (BASE && NT == 1) {
+                            float const* base = p.base_out + at * p.d + g;
+#pragma unroll
+                            for (int i = 0; i < 2 * KS; ++i) bases[i] = i * 8 < p.d - g ? base[i * 8] : 0.f;
+                        }
+                        finish_t const f = finish(m[nt][x], l[nt][x], BASE, BASE ? p.base_lse[at] : 0.f);
                         if (p.lse && g == 0) p.lse[at] = f.lse;
                         if (f.wa == 0.f) { // the sum may be anything
 #pragma unroll
@@ -388,7 +398,14 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                             o[nt][i][x] *= f.wa;
                             o[nt][i][2 + x] *= f.wa;
                         }
-                        if (p.base_out && f.wb != 0.f) {
+                        if (BASE && NT == 1 && f.wb != 0.f) {
+#pragma unroll
+                            for (int i = 0; i < KS; ++i) {
+                                o[nt][i][x] = fmaf(bases[2 * i], f.wb, o[nt][i][x]);
+                                o[nt][i][2 + x] = fmaf(bases[2 * i + 1], f.wb, o[nt][i][2 + x]);
+                            }
+                        }
+                        if (BASE && NT > 1 && f.wb != 0.f) {
                             float const* base = p.base_out + at * p.d + g;
 #pragma unroll
                             for (int i = 0; i < KS; ++i) {
@@ -441,7 +458,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
             mine[2 * lane] = MMA_NO_KEY;
             mine[2 * lane + 1] = 0.f;
         }
-        if (p.base_out) wait_for_base(p);
+        if (BASE) wait_for_base(p);
         __syncthreads();
         uint32_t const start = w.t * TR, count = min((uint32_t)TR, (uint32_t)w.s.n * p.group - start);
         for (uint32_t i = threadIdx.x; i < count * (DPAD / 2); i += THREADS) { // two elements of a row
@@ -465,7 +482,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
             int const      row = w.s.row0 + (int)tok;
             uint32_t const head = w.head * p.group + (pr - tok * p.group);
             uint64_t const at = (uint64_t)row * p.heads + head;
-            finish_t const f = finish(top, l, p.base_lse != nullptr, p.base_lse ? p.base_lse[at] : 0.f);
+            finish_t const f = finish(top, l, BASE, BASE ? p.base_lse[at] : 0.f);
             if (e < p.d) write_out<__half, 2>(p, row, head, e, v, f, true);
             if (e == 0 && p.lse) p.lse[at] = f.lse;
         }
