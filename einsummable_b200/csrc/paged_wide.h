@@ -3,8 +3,8 @@
 //
 // Bound: the tensor cores, and as much the exponentials: a tile of 128 rows x 128 keys of 128 elements is 2 * 512
 // cycles of products and, at 16 exponentials a cycle, 1024 of softmax.  (Measured: 1330 and 1940 with what lies between
-// them, 3500 for the pair of tiles; 256 rows a key head behind 16000 shared tokens 16.9 GF in 30 us, a prompt of 4096
-// tokens with 32 heads 137 GF in 168 us = 0.82 PFLOP/s, where the first tile of a block alone takes 5 us.)  So an item is two tiles of 128 packed rows
+// them, 3500 for the pair of tiles; 256 rows a key head behind 16000 shared tokens 16.9 GF in 31 us, a prompt of 4096
+// tokens with 32 heads 137 GF in 172 us = 0.80 PFLOP/s, where the first tile of a block alone takes 5 us.)  So an item is two tiles of 128 packed rows
 // that share the keys in shared memory and take turns: while one tile's scores are on the tensor cores, the
 // other's are exponentials.  One persistent block an SM, 20 warps:
 //   warps 0-7, 8-15  softmax of tile 0 / 1, two threads a row (= TMEM lane), 64 keys each -- half the
