@@ -8,12 +8,12 @@
 // that share the keys in shared memory and take turns: while one tile's scores are on the tensor cores, the
 // other's are exponentials.  One persistent block an SM, 20 warps:
 //   warps 0-7, 8-15  softmax of tile 0 / 1, two threads a row (= TMEM lane), 64 keys each -- half the
-//                    chain of one thread a row, and half the time results take to leave: exponentials (f32; rounded to
-//                    f16 for the product with the values) against the maximum so far, the maximum of the scores in the
-//                    same pass, both once more and the accumulator rescaled when it has moved by more than 2^8; written
-//                    as f16 pairs over the scores they came from; and the copies of the tile's queries, those of the next item as soon as the last
-//                    scores are there
-//   warp 16          issues the products: S_t = Q_t K^T into TMEM, O_t += P_t V with P_t read from TMEM
+//                    chain of one thread a row, and half the time results take to leave: the maximum of the scores, the
+//                    accumulator rescaled when it has moved by more than 2^8, then the exponentials (f32) against it,
+//                    written as the sum of two f16 over the scores they came from (one f16 rounds by as much as the
+//                    result's type does, and the row's error was 2.9e-4 of the result instead of 2.1e-4); and the copies
+//                    of the tile's queries, those of the next item as soon as the last scores are there
+//   warp 16          issues the products: S_t = Q_t K^T into TMEM, O_t += P_t V with P_t's two parts read from TMEM
 //   warps 17-19      copy the pages into the 128-byte-swizzled tiles the tensor cores read, 16 keys of one page at a
 //                    time (a warp every third 16; one by one where pages are no multiple of 16 tokens, and in the
 //                    sequence's last tile); page numbers are fetched a tile ahead; two stages each for keys and
@@ -307,8 +307,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
             for (uint32_t i = 0; i < 8; ++i) b[i] = b0 + (uint64_t)((i * 2048) >> 4);
             if (leader) {
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) // 16 keys a product: 8 TMEM columns of P (over the scores of its 64 keys), 16 rows of V
-                    umma_ts(d, a0 + (i >> 2) * 64 + (i & 3) * 8, b[i], idesc_o, (keep || i) ? 1u : 0u);
+                for (uint32_t i = 0; i < 8; ++i) { // 16 keys a product: 8 TMEM columns of P's larger, 8 of its smaller parts, 16 rows of V
+                    uint32_t const a = a0 + (i >> 1) * 32 + (i & 1) * 8;
+                    umma_ts(d, a, b[i], idesc_o, (keep || i) ? 1u : 0u);
+                    umma_ts(d, a + 16, b[i], idesc_o, 1u);
+                }
             }
         };
         auto commit = [&](uint32_t b) {
@@ -429,40 +432,28 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     bool const more = j + 1 == f1 && load_next_q();
                     int const  allow = vis - (int)(j * BK + half * 64); // this row sees the first `allow` of the thread's keys
                     bool const mask = __any_sync(0xffffffffu, allow < 64);
-                    // The exponentials are taken against the maximum so far while this tile's is being found: once more
-                    // if it turns out to lie more than 2^8 above that (an item's first tile always; hardly ever another).
-                    // P stays in registers until then: it will lie over the scores.
-                    uint32_t y[32];
-                    uint64_t sum[2];
-#pragma unroll 1
-                    for (int attempt = 0; attempt < 2; ++attempt) {
-                        uint64_t const scale2 = pack2(p.scale_log2, p.scale_log2), m2 = pack2(-m, -m);
-                        float          mx[2] = {-INFINITY, -INFINITY};
-                        sum[0] = sum[1] = 0;
+                    auto       mask_from = [&](uint32_t (&x)[32], int c) { // scores of keys that the row does not see: -inf
+                        if (mask) {
+                            int const here = allow - c * 32;
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t x[32];
-                            tmem_ld32(row_s + c * 32, x);
-                            if (mask) {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    if (c * 32 + i >= allow) x[i] = 0xff800000u; // -inf
-                            }
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                float const s0 = __uint_as_float(x[2 * i]), s1 = __uint_as_float(x[2 * i + 1]);
-                                float       e0, e1;
-                                mx[i & 1] = max3(mx[i & 1], s0, s1);
-                                unpack2(fma2(pack2(s0, s1), scale2, m2), e0, e1);
-                                e0 = ex2(e0);
-                                e1 = ex2(e1);
-                                sum[i & 1] = add2(sum[i & 1], pack2(e0, e1));
-                                y[c * 16 + i] = pack_h2(e0, e1);
-                            }
+                            for (int i = 0; i < 32; ++i)
+                                if (i >= here) x[i] = 0xff800000u;
                         }
-                        float top = fmaxf(mx[0], mx[1]);
-                        top = fmaxf(top, exchange(top)) * p.scale_log2;
-                        if (!__any_sync(0xffffffffu, top > m + MMA_RESCALE)) break; // (the same in both warps)
+                    };
+                    // The tile's maximum first, from one pass over the scores; they are read again for the exponentials, as
+                    // there are no registers for 64 of them.
+                    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t x[32];
+                        tmem_ld32(row_s + c * 32, x);
+                        mask_from(x, c);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) mx[i & 1] = max3(mx[i & 1], __uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+                    }
+                    float top = fmaxf(mx[0], mx[1]);
+                    top = fmaxf(top, exchange(top)) * p.scale_log2;
+                    if (__any_sync(0xffffffffu, top > m + MMA_RESCALE)) { // (the same in both warps)
                         float const mn = fmaxf(m, top), a = ex2(m - mn);
                         m = mn;
                         l *= a;
@@ -477,7 +468,30 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                             }
                         }
                     }
-                    tmem_st32(row_s, y); // (waits for the stores to be done)
+                    // P as the sum of two f16: 16 columns of the larger and 16 of the smaller parts, over the 32 scores they
+                    // came from
+                    uint64_t const scale2 = pack2(p.scale_log2, p.scale_log2), m2 = pack2(-m, -m), minus2 = pack2(-1.f, -1.f);
+                    uint64_t       sum[2] = {0, 0};
+#pragma unroll 1
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t x[32], y[32];
+                        tmem_ld32(row_s + c * 32, x);
+                        mask_from(x, c);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float s0, s1;
+                            unpack2(fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, m2), s0, s1);
+                            s0 = ex2(s0);
+                            s1 = ex2(s1);
+                            uint64_t const e = pack2(s0, s1);
+                            sum[i & 1] = add2(sum[i & 1], e);
+                            y[i] = pack_h2(s0, s1);
+                            float2 const f = __half22float2(*reinterpret_cast<__half2 const*>(&y[i]));
+                            unpack2(fma2(pack2(f.x, f.y), minus2, e), s0, s1);
+                            y[16 + i] = pack_h2(s0, s1);
+                        }
+                        tmem_st32(row_s + c * 32, y); // (waits for the stores to be done)
+                    }
                     tc_fence_before();
                     mbar_arrive(p_ready + 8 * t);
                     float s0, s1;

@@ -330,8 +330,7 @@ int es_b200_launch_cache_append(es_b200_t* h, const es_cache_append_t* a, const 
  * A row that sees no key gets out = 0 and lse = -inf.  Query head h reads key / value head
  * h / (heads / kv_heads).  Any head dim up to 256, any strides; f16 with a head dim that is a multiple of
  * 8 up to 128, strides that are multiples of 8 and 16-byte aligned pointers runs on the tensor cores.
- * f32 accumulation and statistics; where a key head serves more than 16 rows at once (parts of prompts, a
- * batch behind a prefix) the probabilities are rounded to f16 for the product with the values.  A sequence
+ * f32 accumulation and statistics; the tensor cores multiply the probabilities as the sum of two f16.  A sequence
  * without a key to see, NaN and infinities concern the rows that see them only -- and, on the tensor cores, the
  * earlier rows of the same call in the same sequence, for which they are 0 times the value.
  * prefix_len tokens, the same for all sequences and listed by prefix_pages, can lie in front of every

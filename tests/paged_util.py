@@ -3,7 +3,9 @@
 Tolerances are bounds, element by element, from the roundings that the operators are allowed:
   * the result is rounded once to its type: half a step, 2^-11 (f16) or 2^-24 (f32) of the value;
   * on the tensor cores the probabilities are rounded to f16 for the product with the values: 2^-11 of
-    sum_j p_j |v_j| (the sum of the probabilities is not rounded to f16);
+    sum_j p_j |v_j| (the sum of the probabilities is not rounded to f16); with precise=True they are the sum
+    of two f16: 2^-22 of sum_j p_j |v_j|, and as their steps are 2^-24 below 2^-14 and the largest of a row is
+    at least 2^11, 2^-25 / 2^11 of the row's largest probability for each key: 2^-36 max_j p_j sum_j |v_j|;
   * a score is a sum of d products in f32: off by at most (d + 4) 2^-24 scale sum |q_i k_i|; its factor log2 e and
     the subtraction of the maximum add 2^-22 |s| and the exponential 2^-21; a probability's relative error is
     the sum of these, r, and it enters a normalised result twice: 2 r sum_j p_j |v_j|;
@@ -95,14 +97,18 @@ class batch_t:
         return self
 
 
-def truth(b, causal=True, precise=True):
-    """(out, lse, tolerance of out, tolerance of lse), in 64 bits, rows behind the last sequence untouched."""
+def truth(b, causal=True, precise=False):
+    """(out, lse, tolerance of out, tolerance of lse), in 64 bits, rows behind the last sequence untouched.
+    precise: the probabilities are not allowed a single f16's rounding."""
     kc, vc = b.k_cache.cpu().double(), b.v_cache.cpu().double()
     q = b.q.cpu().double()
     out, lse = b.out.cpu().double(), b.lse.cpu().double()
     tol, ltol = torch.zeros_like(out), torch.zeros_like(lse)
     group = b.heads // b.kv_heads
     u, up = UNIT[b.dtype], (UNIT["f16"] if b.dtype == "f16" else 0.0)
+    floor = 0.0
+    if precise and b.dtype == "f16":
+        up, floor = 2.0 ** -22, 2.0 ** -36
     tables, shared = b.tables.cpu().long(), b.prefix_pages.cpu().long()
     for i in range(b.batch):
         for r in range(b.new[i]):
@@ -128,6 +134,9 @@ def truth(b, causal=True, precise=True):
             rel = rel.reshape(b.heads, 1) + sums
             out[row] = o
             tol[row] = u * o.abs() * (1 + 2.0 ** -8) + (up * (1 + 2.0 ** -8) + 2 * rel) * av + (2.0 ** -25 if b.dtype == "f16" else 0)
+            if floor:
+                least = w.amax(-1, keepdim=True) * v.abs().sum(0).unsqueeze(1)  # [kvh, group, dim]
+                tol[row] += floor * least.reshape(b.heads, b.dim)
             lse[row] = torch.logsumexp(s, -1).reshape(b.heads)
             ltol[row] = rel[:, 0] + 2.0 ** -22 * lse[row].abs()
     return out, lse, tol, ltol

@@ -1,0 +1,63 @@
+"""Where the paged-cache operators can go wrong without a random input showing it: rounding that adds up, weights far
+below the largest, what shared memory held before, arrays that are wrong in part, more than one error in a step."""
+import pytest
+import torch
+
+import einsummable_b200 as es
+from paged_util import batch_t, check, truth
+from test_gpu_paged import append_inputs, attend, cache_of, desc_of, km  # noqa: F401 (km: the fixture)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def repeated(b, times):
+    """`times` sequences with the pages, lengths and rows of b's one sequence."""
+    assert b.batch == 1
+    n = b.new[0]
+    b.new, b.total, b.batch = b.new * times, b.total * times, times
+    b.tables, b.lengths = b.tables.repeat(times, 1), b.lengths.repeat(times)
+    b.off = [n * i for i in range(times + 1)]
+    b.used = b.rows = n * times
+    b.row_offsets = torch.tensor(b.off, dtype=torch.int32) if b.row_offsets is not None else None
+    b.q, b.out, b.lse = b.q.repeat(times, 1, 1), b.out.repeat(times, 1, 1), b.lse.repeat(times, 1)
+    return b
+
+
+def set_scores(b, scores, values):
+    """Key j of the one sequence (or of the prefix) gets the score scores[j] from every query, and the value values[j]."""
+    b.scale = 0.125
+    b.q.zero_()
+    b.q[..., 0] = 8
+    n = len(scores)
+    pages = (b.prefix_pages if b.prefix else b.tables[0]).long()
+    at = torch.arange(n)
+    b.k_cache[pages[at // b.page], at % b.page, :, 0] = scores.to(b.k_cache.dtype).unsqueeze(1)
+    b.v_cache[pages[at // b.page], at % b.page] = values.to(b.v_cache.dtype).view(n, 1, 1)
+
+
+@pytest.mark.parametrize("new,past,heads,kv_heads,dim,prefix", [
+    ([1], [2000], 8, 2, 64, 0),                  # single tokens, cut among workers
+    ([1], [900], 8, 2, 128, 0),                  # a block a key head
+    ([1], [2000], 24, 2, 128, 0),                # 12 query heads a key head
+    ([1], [2000], 40, 1, 128, 0),                # 40
+    ([40], [1961], 8, 2, 64, 0),                 # rows of a prompt
+    ([200], [1801], 8, 2, 128, 0),
+    ([1] * 70, [-1] * 70, 8, 2, 128, 4000),      # a batch behind a prefix, read once
+])
+def test_probabilities_are_not_rounded_to_one_f16(km, new, past, heads, kv_heads, dim, prefix):  # noqa: F811
+    """Values of the sign of each probability's rounding to f16: the roundings add up to 2^-13 of the result's
+    magnitude where each is taken once, and the result itself is small, so that its own rounding hides nothing.
+    Every 16th key has the largest score, which is what all kernels measure the others from."""
+    b = batch_t(new, past, heads, kv_heads, dim, 16, prefix=prefix, seed=3)
+    n = prefix or b.total[0]
+    scores = (-0.3 * torch.rand(n, generator=torch.Generator().manual_seed(5))).half().double()
+    scores[::16] = 0
+    e = torch.exp(scores)
+    set_scores(b, scores, torch.where(e.half().double() > e, 1.0, -1.0))
+    want = truth(b, causal=False, precise=True)
+    b.to(DEV)
+    attend(km, b, causal=False)
+    torch.cuda.synchronize()
+    assert km.device_status() == 0
+    check(b, b.out, b.lse, want)
