@@ -10,7 +10,7 @@
 // keys and head dim as the 16 of m16n8k16 and 8 packed rows as its N -- half the matrix instructions, half the
 // accumulators and half the exponentials of 16-row tiles when a key head has up to 8 query heads.  P^T goes from
 // accumulators to the second product through a register transpose.  The running maximum is moved, and the
-// accumulators rescaled, only when a score passes it by more than 2^8: one vote a tile, no reduction.
+// accumulators rescaled, only when a score passes it by more than 2^4: one vote a tile, no reduction.
 // (With 16-row tiles, per-tile maxima and copy addresses formed anew for every copy a tile took 570
 // instructions and 1.6 us a warp, and 64 ragged sequences 117 us.)
 // Measured, 32 query heads on 8 key heads of 128: 2 x 131070 keys (1.07 GB) 171-176 us = 6.1-6.3 TB/s, 64 sequences of
@@ -24,7 +24,10 @@ namespace es {
 namespace {
 
 constexpr int MMA_BK = 16, MMA_OVH = 6, MMA_WARPS = 4, MMA_STAGES = 3;
-constexpr float MMA_RESCALE = 8.f;
+// Exponentials are taken 2^11 times as large: f16 has steps of 2^-24 below 2^-14, and what is lost of a weight there
+// is then 2^-36 of the largest instead of 2^-25, which put 30000 small weights behind a large one of value 0
+// off by 0.6 %.  2^11 x 2^4, what the maximum may be passed by, stays within f16.
+constexpr float MMA_LIFT = 11.f, MMA_RESCALE = 4.f;
 constexpr float MMA_NO_KEY = -1e30f; // the maximum before the first key: finite, so that no difference is inf - inf
 
 template <int OFF> __device__ __forceinline__ void copy16_at(uint32_t dst, void const* src)
@@ -288,8 +291,8 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        s[nt][1][i] = fmaf(s[nt][0][i], p.scale_log2, -m[nt][i & 1]);
-                        over |= s[nt][1][i] > MMA_RESCALE;
+                        s[nt][1][i] = fmaf(s[nt][0][i], p.scale_log2, MMA_LIFT - m[nt][i & 1]);
+                        over |= s[nt][1][i] > MMA_LIFT + MMA_RESCALE;
                     }
                 if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -308,8 +311,8 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                                 o[nt][i][x] *= a;
                                 o[nt][i][2 + x] *= a;
                             }
-                            s[nt][1][x] = fmaf(s[nt][0][x], p.scale_log2, -mn);
-                            s[nt][1][2 + x] = fmaf(s[nt][0][2 + x], p.scale_log2, -mn);
+                            s[nt][1][x] = fmaf(s[nt][0][x], p.scale_log2, MMA_LIFT - mn);
+                            s[nt][1][2 + x] = fmaf(s[nt][0][2 + x], p.scale_log2, MMA_LIFT - mn);
                         }
                 }
                 uint32_t b[NT][2], low[NT][2];
@@ -343,6 +346,10 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                 }
                 st = st + stage_bytes == ring_end ? ring : st + stage_bytes;
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) // what the sums are relative to
+#pragma unroll
+                for (int x = 0; x < 2; ++x) m[nt][x] -= MMA_LIFT;
             if (p.direct == DIRECT_BLOCK) { // into this warp's ring, which is done with: maxima and sums, then the rows
                 __syncwarp();
 #pragma unroll

@@ -9,7 +9,7 @@
 // other's are exponentials.  One persistent block an SM, 20 warps:
 //   warps 0-7, 8-15  softmax of tile 0 / 1, two threads a row (= TMEM lane), 64 keys each -- half the
 //                    chain of one thread a row, and half the time results take to leave: the maximum of the scores, the
-//                    accumulator rescaled when it has moved by more than 2^8, then the exponentials (f32) against it,
+//                    accumulator rescaled when it has moved by more than 2^4, then the exponentials (f32) against it,
 //                    written as the sum of two f16 over the scores they came from (one f16 rounds by as much as the
 //                    result's type does, and the row's error was 2.9e-4 of the result instead of 2.1e-4); and the copies
 //                    of the tile's queries, those of the next item as soon as the last scores are there
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     }
                     // P as the sum of two f16: 16 columns of the larger and 16 of the smaller parts, over the 32 scores they
                     // came from
-                    uint64_t const scale2 = pack2(p.scale_log2, p.scale_log2), m2 = pack2(-m, -m), minus2 = pack2(-1.f, -1.f);
+                    uint64_t const scale2 = pack2(p.scale_log2, p.scale_log2), m2 = pack2(MMA_LIFT - m, MMA_LIFT - m), minus2 = pack2(-1.f, -1.f);
                     uint64_t       sum[2] = {0, 0};
 #pragma unroll 1
                     for (int c = 0; c < 2; ++c) {
@@ -499,6 +499,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     l += s0 + s1;
                     if (more) tell_q();
                 }
+                m -= MMA_LIFT; // what the sums are relative to
                 float const others = exchange(l);
                 l = half ? others + l : l + others; // (the same sum in both)
                 if (f1 > f0) {

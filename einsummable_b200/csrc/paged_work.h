@@ -40,7 +40,7 @@ struct paged_params_t {
     float const*   base_out;    // result over a prefix [rows, heads, d], merged in; may be null
     float const*   base_lse;
     float*         part_out;    // [workers][2][TR][part_d]
-    float2*        part_ml;     // [workers][2][TR]: maximum (log2 units), sum
+    float2*        part_ml;     // [workers][2][TR]: what the sum is relative to (log2 units), sum
     int4*          meta;        // [workers][2]
     int64_t        q_stride[2], out_stride[2], k_stride[3], v_stride[3];
     uint32_t       batch, rows, heads, kv_heads, group, d, part_d, n_pages, table_stride, capacity;

@@ -61,3 +61,24 @@ def test_probabilities_are_not_rounded_to_one_f16(km, new, past, heads, kv_heads
     torch.cuda.synchronize()
     assert km.device_status() == 0
     check(b, b.out, b.lse, want)
+
+
+@pytest.mark.parametrize("new,heads,kv_heads,times", [
+    (1, 32, 8, 160),   # single tokens: more (sequence, key head)s than workers, so that one worker has a whole one
+    (8, 32, 1, 150),   # 256 rows a key head: more than there are blocks
+])
+def test_many_keys_far_below_one_that_dominates(km, new, heads, kv_heads, times):  # noqa: F811
+    """One key with all of the weight and a value of 0, and 30000 keys 15 to 17 below it (weights of 2^-22 to 2^-25)
+    that make up the result."""
+    n = 30000
+    b = batch_t([new], [n - new], heads, kv_heads, 64, 16, seed=4, offsets=new > 1)
+    scores = (-15 - 2 * torch.rand(n, generator=torch.Generator().manual_seed(6))).half().double()
+    values = torch.ones(n)
+    scores[0], values[0] = 0, 0
+    set_scores(b, scores, values)
+    out, lse, tol, ltol = truth(b, causal=False, precise=True)
+    repeated(b, times).to(DEV)
+    attend(km, b, causal=False)
+    torch.cuda.synchronize()
+    assert km.device_status() == 0
+    check(b, b.out, b.lse, tuple(x.repeat(times, *[1] * (x.dim() - 1)) for x in (out, lse, tol, ltol)))
