@@ -247,10 +247,11 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                 asm volatile("cp.async.wait_group %0;" ::"n"(MMA_STAGES - 2) : "memory");
                 __syncwarp(); // the other lanes' copies too; and the stage that issue() fills next has been read
                 if (u == 0) {
-                    // B operand of K Q^T: 8 rows x 32 elements a load
+                    // B operand of K Q^T: 8 rows x 32 elements a load.  Rows that the item lacks are its last one once more: what
+                    // lies in their place is left from other kernels, and would take part in the vote on the maximum
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        uint32_t const r = min((uint32_t)(nt * 8 + l7), q_rows - 1);
+                        uint32_t const r = min((uint32_t)(nt * 8 + l7), count - 1);
 #pragma unroll
                         for (int i = 0; i < KS / 2; ++i) {
                             uint32_t t[4];

@@ -82,3 +82,24 @@ def test_many_keys_far_below_one_that_dominates(km, new, heads, kv_heads, times)
     torch.cuda.synchronize()
     assert km.device_status() == 0
     check(b, b.out, b.lse, tuple(x.repeat(times, *[1] * (x.dim() - 1)) for x in (out, lse, tol, ltol)))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("prefix", [0, 900])
+def test_the_same_bits_whatever_ran_before(km, dim, prefix):  # noqa: F811
+    """Single tokens with row offsets: 4 of a tile's 8 query rows do not exist.  Calls whose tiles are full, with
+    queries that move the maximum all the time or not at all, leave their rows in shared memory."""
+    past = [3000, 10, 700, 64, 1999, 830, 1500, 411]
+    b = batch_t([1] * 8, past, 8, 2, dim, 16, seed=6, offsets=True, prefix=prefix).to(DEV)
+    before = batch_t([2] * 8, past, 8, 2, dim, 16, seed=7, offsets=True, prefix=prefix).to(DEV)
+    seen = []
+    for factor in (0, 100, 0, 1000, 30):
+        keep = before.q.clone()
+        before.q *= factor
+        attend(km, before)
+        before.q = keep
+        attend(km, b)
+        torch.cuda.synchronize()
+        seen.append((b.out.clone(), b.lse.clone()))
+    for out, lse in seen[1:]:
+        assert torch.equal(out, seen[0][0]) and torch.equal(lse, seen[0][1])
