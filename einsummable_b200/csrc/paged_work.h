@@ -92,18 +92,26 @@ struct sequence_t {
     int32_t const* table;
 };
 
-__device__ __forceinline__ sequence_t get_sequence(paged_params_t const& p, uint32_t i)
+// Rows that attend a prefix: up to where the last sequence ends.  When the offsets are wrong (some sequence ends behind
+// that, or it lies outside the tensors) all rows there are, as the good sequences may lie anywhere among them.  All
+// threads of the block call.
+__device__ __forceinline__ uint32_t prefix_rows(paged_params_t const& p)
+{
+    if (!p.row_offsets) return p.rows;
+    int const end = p.row_offsets[p.batch];
+    bool      ok = end >= 0 && end <= (int)p.rows;
+    for (uint32_t i = threadIdx.x; i < p.batch; i += blockDim.x) ok = ok && p.row_offsets[i] <= end;
+    if (__syncthreads_and(ok)) return (uint32_t)end;
+    if (threadIdx.x == 0) report(p, PAGED_BAD_ROWS);
+    return p.rows;
+}
+
+// rows: of a prefix (prefix_rows)
+__device__ __forceinline__ sequence_t get_sequence(paged_params_t const& p, uint32_t i, uint32_t rows = 0)
 {
     sequence_t s;
     if (p.prefix_len >= 0) {
-        s.n = (int)p.rows;
-        if (p.row_offsets) {
-            s.n = p.row_offsets[p.batch];
-            if (s.n < 0 || s.n > (int)p.rows) {
-                report(p, PAGED_BAD_ROWS);
-                s.n = 0;
-            }
-        }
+        s.n = (int)rows;
         s.len = p.prefix_len;
         s.row0 = 0;
         s.table = p.tables;
@@ -228,12 +236,13 @@ __device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sc
         }
         return;
     }
-    uint64_t   mine = 0, u0 = 0;
+    uint32_t const rows = p.prefix_len >= 0 ? prefix_rows(p) : 0;
+    uint64_t       mine = 0, u0 = 0;
     for (uint32_t i0 = 0; i0 < n_seq; i0 += NT) {
         sequence_t s;
         s.n = 0;
         s.len = 0;
-        if (i0 + threadIdx.x < n_seq) s = get_sequence(p, i0 + threadIdx.x);
+        if (i0 + threadIdx.x < n_seq) s = get_sequence(p, i0 + threadIdx.x, rows);
         u0 = head_units<TR, BK, OVH>(p, s) * p.kv_heads;
         mine += u0;
     }
@@ -259,7 +268,7 @@ __device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sc
             sequence_t s;
             s.n = 0;
             s.len = 0;
-            if (i0 + threadIdx.x < n_seq) s = get_sequence(p, i0 + threadIdx.x);
+            if (i0 + threadIdx.x < n_seq) s = get_sequence(p, i0 + threadIdx.x, rows);
             u = head_units<TR, BK, OVH>(p, s) * p.kv_heads;
         }
         uint64_t incl = u;
@@ -294,7 +303,7 @@ __device__ __forceinline__ void find_work(paged_params_t const& p, work_t& w, sc
     w.left = (uint32_t)min((uint64_t)w.chunk, total - lo);
     w.seq = sm.found_seq[mine_in_block];
     uint64_t off = sm.found_off[mine_in_block];
-    w.s = get_sequence(p, w.seq);
+    w.s = get_sequence(p, w.seq, rows);
     uint64_t const per_head = head_units<TR, BK, OVH>(p, w.s); // every lane of every warp has the same sequence
     w.head = (uint32_t)(off / per_head);
     off -= w.head * per_head;

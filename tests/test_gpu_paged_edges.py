@@ -103,3 +103,23 @@ def test_the_same_bits_whatever_ran_before(km, dim, prefix):  # noqa: F811
         seen.append((b.out.clone(), b.lse.clone()))
     for out, lse in seen[1:]:
         assert torch.equal(out, seen[0][0]) and torch.equal(lse, seen[0][1])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("prefix", [0, 70, 700])
+@pytest.mark.parametrize("many", [1, 30])
+def test_bad_row_offsets_leave_the_other_sequences_right(km, dtype, prefix, many):  # noqa: F811
+    for off, valid in [([0, 2, 5, 99], [0, 1]), ([0, 2, 5, 3], [0, 1]), ([-1, 2, 3, 5], [1, 2]), ([0, 2, 2 ** 20, 5], [0]),
+                       ([0, 2, 5, -7], [0, 1]), ([0, 3, 1, 0], [0])]:
+        off = [x * many for x in off]
+        b = batch_t([2 * many, many, 2 * many], [40, 200, 90], 8, 2, 64, 16, dtype=dtype, seed=9, prefix=prefix)
+        b.new = [off[i + 1] - off[i] if i in valid else 0 for i in range(3)]
+        b.off = off
+        rows = [r for i in valid for r in range(off[i], off[i + 1])]
+        want = truth(b)
+        b.to(DEV)
+        b.row_offsets = torch.tensor(off, dtype=torch.int32, device=DEV)
+        attend(km, b)
+        torch.cuda.synchronize()
+        assert km.device_status() == 0x23
+        check(b, b.out[rows], b.lse[rows], tuple(x[rows] for x in want))
