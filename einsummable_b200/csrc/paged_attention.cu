@@ -279,7 +279,9 @@ void check_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
     if (!a.heads || a.heads % c.kv_heads) fail(ES_BAD_DESCRIPTOR, "paged attention: query heads must be a multiple of the key heads");
     if (a.heads > 65535) fail(ES_NOT_SUPPORTED, "paged attention: more than 65535 heads");
     if ((uint64_t)c.rows * (a.heads / c.kv_heads) > 0x7fffffffull) fail(ES_NOT_SUPPORTED, "paged attention: too many rows");
-    if (!(a.scale >= 1e-30f && a.scale <= 1e30f)) fail(ES_BAD_DESCRIPTOR, "paged attention: the scale must lie in 1e-30 .. 1e30");
+    // (f16: 256 * 65504^2 * 1e26 * log2 e, so that every score and lse is finite)
+    if (!(a.scale >= 1e-30f && a.scale <= (c.dtype == ES_F16 ? 1e26f : 1e30f)))
+        fail(ES_BAD_DESCRIPTOR, "paged attention: the scale must lie in 1e-30 .. 1e30 (f16: 1e26)");
     if (!x.q || !x.k_cache || !x.v_cache || !x.out || !x.lengths || !x.tables) fail(ES_BAD_ARGUMENT, "paged attention: null pointer");
     if (!prefix && a.prefix_len) fail(ES_BAD_ARGUMENT, "paged attention: a prefix needs es_b200_launch_prefix_attention");
     if (a.prefix_len > MAX_TOKENS) fail(ES_NOT_SUPPORTED, "paged attention: prefix beyond 2^30 tokens");

@@ -28,7 +28,10 @@ constexpr int MMA_BK = 16, MMA_OVH = 6, MMA_WARPS = 4, MMA_STAGES = 3;
 // is then 2^-36 of the largest instead of 2^-25, which put 30000 small weights behind a large one of value 0
 // off by 0.6 %.  2^11 x 2^4, what the maximum may be passed by, stays within f16.
 constexpr float MMA_LIFT = 11.f, MMA_RESCALE = 4.f;
-constexpr float MMA_NO_KEY = -1e30f; // the maximum before the first key: finite, so that no difference is inf - inf
+// The maximum is kept in units of the scores and subtracted before they are scaled: the difference of near scores is
+// exact, and that of the largest from itself 0, however large they are (against a scaled and rounded maximum the
+// exponentials of scores beyond 2^28 were infinite).
+constexpr float MMA_NO_KEY = -1e37f; // the maximum before the first key: below all f16 scores, and finite: no inf - inf
 
 template <int OFF> __device__ __forceinline__ void copy16_at(uint32_t dst, void const* src)
 {
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        s[nt][1][i] = fmaf(s[nt][0][i], p.scale_log2, MMA_LIFT - m[nt][i & 1]);
+                        s[nt][1][i] = fmaf(s[nt][0][i] - m[nt][i & 1], p.scale_log2, MMA_LIFT);
                         over |= s[nt][1][i] > MMA_LIFT + MMA_RESCALE;
                     }
                 if (__any_sync(0xffffffffu, over)) {
@@ -300,11 +303,11 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            float mx = fmaxf(s[nt][0][x] * p.scale_log2, s[nt][0][2 + x] * p.scale_log2);
+                            float mx = fmaxf(s[nt][0][x], s[nt][0][2 + x]);
 #pragma unroll
                             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
                             float const mn = fmaxf(m[nt][x], mx);
-                            float const a = ex2(m[nt][x] - mn);
+                            float const a = ex2((m[nt][x] - mn) * p.scale_log2);
                             m[nt][x] = mn;
                             l[nt][x] *= a;
 #pragma unroll
@@ -312,8 +315,8 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                                 o[nt][i][x] *= a;
                                 o[nt][i][2 + x] *= a;
                             }
-                            s[nt][1][x] = fmaf(s[nt][0][x], p.scale_log2, MMA_LIFT - mn);
-                            s[nt][1][2 + x] = fmaf(s[nt][0][2 + x], p.scale_log2, MMA_LIFT - mn);
+                            s[nt][1][x] = fmaf(s[nt][0][x] - mn, p.scale_log2, MMA_LIFT);
+                            s[nt][1][2 + x] = fmaf(s[nt][0][2 + x] - mn, p.scale_log2, MMA_LIFT);
                         }
                 }
                 uint32_t b[NT][2], low[NT][2];
@@ -348,9 +351,9 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, 2) paged_mma_kernel(const __gr
                 st = st + stage_bytes == ring_end ? ring : st + stage_bytes;
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) // what the sums are relative to
+            for (int nt = 0; nt < NT; ++nt) // what the sums are relative to, in log2 units
 #pragma unroll
-                for (int x = 0; x < 2; ++x) m[nt][x] -= MMA_LIFT;
+                for (int x = 0; x < 2; ++x) m[nt][x] = fmaf(m[nt][x], p.scale_log2, -MMA_LIFT);
             if (p.direct == DIRECT_BLOCK) { // into this warp's ring, which is done with: maxima and sums, then the rows
                 __syncwarp();
 #pragma unroll

@@ -452,9 +452,9 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                         for (int i = 0; i < 16; ++i) mx[i & 1] = max3(mx[i & 1], __uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
                     }
                     float top = fmaxf(mx[0], mx[1]);
-                    top = fmaxf(top, exchange(top)) * p.scale_log2;
-                    if (__any_sync(0xffffffffu, top > m + MMA_RESCALE)) { // (the same in both warps)
-                        float const mn = fmaxf(m, top), a = ex2(m - mn);
+                    top = fmaxf(top, exchange(top));
+                    if (__any_sync(0xffffffffu, (top - m) * p.scale_log2 > MMA_RESCALE)) { // (the same in both warps)
+                        float const mn = fmaxf(m, top), a = ex2((m - mn) * p.scale_log2);
                         m = mn;
                         l *= a;
                         if (j != f0) {
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     }
                     // P as the sum of two f16: 16 columns of the larger and 16 of the smaller parts, over the 32 scores they
                     // came from
-                    uint64_t const scale2 = pack2(p.scale_log2, p.scale_log2), m2 = pack2(MMA_LIFT - m, MMA_LIFT - m), minus2 = pack2(-1.f, -1.f);
+                    uint64_t const scale2 = pack2(p.scale_log2, p.scale_log2), lift2 = pack2(MMA_LIFT, MMA_LIFT), m2 = pack2(-m, -m), minus2 = pack2(-1.f, -1.f);
                     uint64_t       sum[2] = {0, 0};
 #pragma unroll 1
                     for (int c = 0; c < 2; ++c) {
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             float s0, s1;
-                            unpack2(fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, m2), s0, s1);
+                            unpack2(fma2(add2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), m2), scale2, lift2), s0, s1);
                             s0 = ex2(s0);
                             s1 = ex2(s1);
                             uint64_t const e = pack2(s0, s1);
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
                     l += s0 + s1;
                     if (more) tell_q();
                 }
-                m -= MMA_LIFT; // what the sums are relative to
+                m = fmaf(m, p.scale_log2, -MMA_LIFT); // what the sums are relative to, in log2 units
                 float const others = exchange(l);
                 l = half ? others + l : l + others; // (the same sum in both)
                 if (f1 > f0) {

@@ -343,7 +343,7 @@ typedef struct {
     es_paged_cache_t cache; /* dtype also of q and out */
     uint32_t heads;         /* a multiple of cache.kv_heads */
     int32_t  causal;
-    float    scale;         /* 1e-30 .. 1e30 */
+    float    scale;         /* 1e-30 .. 1e30 (f16: 1e26) */
     uint32_t prefix_len;
     int64_t  q_stride[2], out_stride[2]; /* elements: row, head */
 } es_paged_attention_t;

@@ -123,3 +123,27 @@ def test_bad_row_offsets_leave_the_other_sequences_right(km, dtype, prefix, many
         torch.cuda.synchronize()
         assert km.device_status() == 0x23
         check(b, b.out[rows], b.lse[rows], tuple(x[rows] for x in want))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (24, 2), (40, 1)])
+@pytest.mark.parametrize("scale", [1.0, 1e26])
+def test_scores_of_any_size(km, heads, kv_heads, scale):  # noqa: F811
+    """Scores of -2 x 10^11 and of -2 x 10^37, the largest that f16 and the scale allow: the one nearest to 0 has all
+    of the weight."""
+    b = batch_t([1, 1], [300, 40], heads, kv_heads, 64, 16, seed=8)
+    b.scale = scale
+    b.q.fill_(60000)
+    want = torch.zeros_like(b.out)
+    for i in range(2):
+        at = torch.arange(b.total[i])
+        pages = b.tables[i].long()
+        b.k_cache[pages[at // 16], at % 16] = -60000.0
+        b.k_cache[pages[27 // 16], 27 % 16] = -59008.0
+        want[i] = b.v_cache[pages[27 // 16], 27 % 16].repeat_interleave(heads // kv_heads, 0)
+    b.to(DEV)
+    attend(km, b)
+    torch.cuda.synchronize()
+    assert km.device_status() == 0
+    assert torch.equal(b.out.cpu(), want)
+    top = -64 * 60000.0 * 59008.0 * scale
+    assert ((b.lse.cpu().double() / top - 1).abs() <= 2.0 ** -17).all()  # 64 sums, scale, log2 e, ln 2: 2^-24 each
