@@ -570,15 +570,15 @@ int es_b200_device_status(es_b200_t* h, unsigned int* error_word)
         if (!error_word) fail(ES_BAD_ARGUMENT, "null pointer");
         set_device(h);
         ES_CUDA_CHECK(cudaDeviceSynchronize());
-        unsigned int tc = read_and_clear_tc_error();
-        unsigned int at = read_and_clear_attention_error();
-        if (!tc) tc = at;
-        unsigned int ap = read_and_clear_append_error();
-        unsigned int pg = read_and_clear_paged_error();
-        if (!tc) tc = ap ? ap : pg;
-        unsigned int fl = read_and_clear_flag_error();
-        unsigned int ex = read_and_clear_exchange_error();
-        *error_word = tc | ((fl ? fl : ex) << 8);
+        // each byte one word at a time, waits that expired (whose output is not valid) before what the append found in its
+        // arrays: a word that is not reported stays for the next call
+        unsigned int low = read_and_clear_tc_error();
+        if (!low) low = read_and_clear_attention_error();
+        if (!low) low = read_and_clear_paged_error();
+        if (!low) low = read_and_clear_append_error();
+        unsigned int high = read_and_clear_flag_error();
+        if (!high) high = read_and_clear_exchange_error();
+        *error_word = low | (high << 8);
     });
 }
 

@@ -82,7 +82,7 @@ __device__ __forceinline__ void wait_for_base(paged_params_t const& p)
 
 __device__ __forceinline__ void report(paged_params_t const& p, unsigned code)
 {
-    atomicCAS(p.error, 0u, code);
+    atomicMax(p.error, code); // a wait that expired (0x31..) passes what the arrays hold (0x21..)
 }
 
 struct sequence_t {

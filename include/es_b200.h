@@ -406,12 +406,12 @@ int es_b200_rowsum_f32_noalloc(es_b200_t*   h,
                                uint64_t     cols,
                                void*        stream);
 
-/* Synchronises the device and returns (and clears) the error word of the
- * tensor-core kernels: 0 = fine; nonzero = a bounded wait inside a kernel gave
- * up (1 producer, 2/3 MMA issuer, 4 epilogue) and that launch's output is not
- * valid; 0x11..0x16 = the same inside the attention kernel (Q copy, K copy, scores, P tile,
- * V copy, P V), 0x21..0x24 = what a paged-cache kernel found in its arrays, 0x31..0x39 = a wait inside
- * the paged attention kernel.  The reference has no counterpart: its library kernels cannot report. */
+/* Synchronises the device and returns (and clears) an error word of the kernels: 0 = fine; nonzero = a
+ * bounded wait inside a tensor-core kernel gave up (1 producer, 2/3 MMA issuer, 4 epilogue) and that
+ * launch's output is not valid; 0x11..0x16 = the same inside the attention kernel (Q copy, K copy,
+ * scores, P tile, V copy, P V), 0x31..0x39 = inside the paged attention kernel; 0x21..0x24 = what a
+ * paged-cache kernel found in its arrays.  When kernels of several kinds have recorded one, the next call
+ * returns the next.  The reference has no counterpart: its library kernels cannot report. */
 int es_b200_device_status(es_b200_t* h, unsigned int* error_word);
 
 /* Clock trace of the tensor-core contraction kernel (trace builds only: the library compiled

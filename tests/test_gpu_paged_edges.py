@@ -147,3 +147,18 @@ def test_scores_of_any_size(km, heads, kv_heads, scale):  # noqa: F811
     assert torch.equal(b.out.cpu(), want)
     top = -64 * 60000.0 * 59008.0 * scale
     assert ((b.lse.cpu().double() / top - 1).abs() <= 2.0 ** -17).all()  # 64 sums, scale, log2 e, ln 2: 2^-24 each
+
+
+def test_every_error_of_a_step_is_reported(km):  # noqa: F811
+    """An append with a bad length and an attention with a bad page: one after the other, whichever came first."""
+    assert km.device_status() == 0
+    b = batch_t([1, 1], [40, 200], 8, 2, 64, 16, seed=9).to(DEV)
+    b.tables[1, 3] = b.n_pages
+    attend(km, b)
+    x = torch.zeros((2, 2, 64), dtype=torch.float16, device=DEV)
+    d = es.cache_append_t(cache_of(b), "f16", 0, k_stride=x.stride()[:2], v_stride=x.stride()[:2])
+    lengths = torch.tensor([-3, 0], dtype=torch.int32, device=DEV)
+    km.cache_append(d, None, b.k_cache, b.v_cache, x, x, lengths, b.tables)
+    torch.cuda.synchronize()
+    assert sorted([km.device_status(), km.device_status()]) == [0x21, 0x22]
+    assert km.device_status() == 0
