@@ -33,7 +33,7 @@ def _ptr(x):
         raise TypeError("expected a device pointer (int) or a torch tensor") from None
 
 
-def _adr(x):
+def _adr(x):  # (a null pointer is the library's to refuse, or to take)
     return 0 if x is None else _ptr(x)
 
 
@@ -215,8 +215,8 @@ class kernel_manager_t:
         rotated into q_out.  `desc` is a cache_append_t (einsummable_b200.paged); lengths [batch] count the new
         tokens already, tables [batch, table_stride] and row_offsets [batch + 1] (None: one row a sequence) are
         int32 on the device, freqs the complex64 table [n_positions, rotary_dim / 2]."""
-        x = _pack10(_adr(q), _ptr(k), _ptr(v), _adr(freqs), _adr(q_out), _ptr(k_cache), _ptr(v_cache), _adr(row_offsets),
-                    _ptr(lengths), _ptr(tables))
+        x = _pack10(_adr(q), _adr(k), _adr(v), _adr(freqs), _adr(q_out), _adr(k_cache), _adr(v_cache), _adr(row_offsets),
+                    _adr(lengths), _adr(tables))
         _lib.check(self._lib.es_b200_launch_cache_append(self._h, desc.ref, x, _stream(stream)))
 
     def paged_attention_workspace(self, desc):
@@ -230,7 +230,7 @@ class kernel_manager_t:
         """Attention of the step's queries to their own sequences' keys in the cache; lse [rows, heads] f32 gets
         the logarithm of the sums of exponentials.  `desc` is a paged_attention_t (einsummable_b200.paged), the
         arrays as for cache_append, workspace = (device memory, bytes)."""
-        x = _pack9(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _adr(lse), _adr(row_offsets), _ptr(lengths), _ptr(tables), 0)
+        x = _pack9(_adr(q), _adr(k_cache), _adr(v_cache), _adr(out), _adr(lse), _adr(row_offsets), _adr(lengths), _adr(tables), 0)
         ws, n = (None, 0) if workspace is None else (_ptr(workspace[0]), int(workspace[1]))
         _lib.check(self._lib.es_b200_launch_paged_attention(self._h, desc.ref, x, ws, n, _stream(stream)))
 
@@ -238,7 +238,7 @@ class kernel_manager_t:
                          lse=None, workspace=None):
         """The same behind a prefix that all sequences share: its desc.prefix_len tokens lie in the pages
         prefix_pages (int32 on the device) and are read once for the whole batch."""
-        x = _pack9(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _adr(lse), _adr(row_offsets), _ptr(lengths), _ptr(tables),
+        x = _pack9(_adr(q), _adr(k_cache), _adr(v_cache), _adr(out), _adr(lse), _adr(row_offsets), _adr(lengths), _adr(tables),
                    _adr(prefix_pages))
         ws, n = (None, 0) if workspace is None else (_ptr(workspace[0]), int(workspace[1]))
         _lib.check(self._lib.es_b200_launch_prefix_attention(self._h, desc.ref, x, ws, n, _stream(stream)))

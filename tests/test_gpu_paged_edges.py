@@ -162,3 +162,21 @@ def test_every_error_of_a_step_is_reported(km):  # noqa: F811
     torch.cuda.synchronize()
     assert sorted([km.device_status(), km.device_status()]) == [0x21, 0x22]
     assert km.device_status() == 0
+
+
+def test_null_tensors_are_refused(km):  # noqa: F811
+    b = batch_t([1], [40], 4, 2, 64, 16, seed=1).to(DEV)
+    n = km.paged_attention_workspace(desc_of(b))
+    ws = (torch.empty(n, dtype=torch.uint8, device=DEV), n)
+    args = [b.out, b.q, b.k_cache, b.v_cache, b.lengths, b.tables]
+    for i in range(6):
+        with pytest.raises(es.es_error) as e:
+            km.paged_attention(desc_of(b), None, *[None if j == i else a for j, a in enumerate(args)], workspace=ws)
+        assert e.value.status == 6
+    k = torch.zeros((1, 2, 64), dtype=torch.float16, device=DEV)
+    d = es.cache_append_t(cache_of(b), "f16", 0, k_stride=k.stride()[:2], v_stride=k.stride()[:2])
+    args = [b.k_cache, b.v_cache, k, k, b.lengths, b.tables]
+    for i in range(6):
+        with pytest.raises(es.es_error) as e:
+            km.cache_append(d, None, *[None if j == i else a for j, a in enumerate(args)])
+        assert e.value.status == 6

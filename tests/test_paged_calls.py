@@ -3,7 +3,25 @@ import pytest
 
 import einsummable_b200 as es
 from einsummable_b200 import _lib
-from test_paged import add_attention, attention, cache
+from test_paged import PTR, add_attention, append, attention, cache
+
+
+@pytest.fixture
+def km():
+    m = es.kernel_manager_t.__new__(es.kernel_manager_t)  # no device: every call ends at the handle at the latest
+    m._lib, m._h = _lib.load(), None
+    yield m
+    m._h = None
+
+
+@pytest.mark.parametrize("missing", range(6))
+def test_none_for_a_tensor_is_refused_by_the_library(km, missing):
+    six = [None if i == missing else PTR for i in range(6)]
+    for call in (lambda: km.paged_attention(attention(), None, *six), lambda: km.cache_append(append(), None, *six),
+                 lambda: km.prefix_attention(attention(prefix_len=3), None, *six[:4], PTR, *six[4:])):
+        with pytest.raises(es.es_error) as e:
+            call()
+        assert e.value.status == _lib.ES_BAD_ARGUMENT
 
 
 @pytest.mark.parametrize("dtype,most", [("f16", 1e26), ("f32", 1e30)])
