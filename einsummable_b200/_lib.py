@@ -116,10 +116,10 @@ SYMBOLS = {
     "es_b200_flag_wait": (_i, [_vp, _vp, ctypes.c_uint32, _vp]),
     "es_b200_pull": (_i, [_vp, _vp, _vp, _u64, _vp]),
     "es_b200_launch_attention": (_i, [_vp, ctypes.POINTER(es_attention_t), _vp, _vp, _vp, _vp, _vp, _vp]),
-    "es_b200_launch_cache_append": (_i, [_vp, _vp, _vp, _vp]),
+    "es_b200_launch_cache_append": (_i, [_vp, ctypes.POINTER(es_cache_append_t), _vp, _vp]),
     "es_b200_paged_attention_workspace": (_i, [ctypes.POINTER(es_paged_attention_t), ctypes.POINTER(_u64)]),
-    "es_b200_launch_paged_attention": (_i, [_vp, _vp, _vp, _vp, _u64, _vp]),
-    "es_b200_launch_prefix_attention": (_i, [_vp, _vp, _vp, _vp, _u64, _vp]),
+    "es_b200_launch_paged_attention": (_i, [_vp, ctypes.POINTER(es_paged_attention_t), _vp, _vp, _u64, _vp]),
+    "es_b200_launch_prefix_attention": (_i, [_vp, ctypes.POINTER(es_paged_attention_t), _vp, _vp, _u64, _vp]),
     "es_b200_kernel_info": (_i, [_vp, _u64, _cp, _i]),
     "es_b200_describe": (_i, [_desc_p, _i, _cp, _i]),
     "es_b200_touch_simplify": (_i, [_td_p, _i, _td_p, ctypes.POINTER(_i)]),

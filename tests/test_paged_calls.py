@@ -1,4 +1,6 @@
 """The calls of the paged cache without a GPU: arguments that never reach a kernel."""
+import ctypes
+
 import pytest
 
 import einsummable_b200 as es
@@ -22,6 +24,15 @@ def test_none_for_a_tensor_is_refused_by_the_library(km, missing):
         with pytest.raises(es.es_error) as e:
             call()
         assert e.value.status == _lib.ES_BAD_ARGUMENT
+
+
+def test_descriptors_are_not_taken_for_one_another(km):
+    """A descriptor of the other kind is shorter or longer than what the library would read."""
+    six = [PTR] * 6
+    for call in (lambda: km.paged_attention(append(), None, *six), lambda: km.cache_append(attention(), None, *six),
+                 lambda: km.prefix_attention(append(), None, *six, PTR), lambda: km.paged_attention_workspace(append())):
+        with pytest.raises((TypeError, ctypes.ArgumentError)):
+            call()
 
 
 @pytest.mark.parametrize("dtype,most", [("f16", 1e26), ("f32", 1e30)])
