@@ -148,11 +148,12 @@ template <bool HALVES, bool VEC, typename T> __device__ __forceinline__ void sto
         store_n<4, VEC>(p + t.e1, b, t.n1);
     }
 }
-// c: cosine and sine of the unit's four pairs
-template <bool HALVES> __device__ __forceinline__ void rotate(float (&x)[8], float const (&c)[8])
+// c: cosine and sine of the unit's four pairs, of which the first n are rotated
+template <bool HALVES> __device__ __forceinline__ void rotate(float (&x)[8], float const (&c)[8], int n)
 {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+        if (j >= n) break; // (by a factor of 1 + 0 i an infinity would become its neighbour's NaN)
         int const   i0 = HALVES ? j : 2 * j, i1 = HALVES ? 4 + j : 2 * j + 1;
         float const a = x[i0], b = x[i1];
         x[i0] = a * c[2 * j] - b * c[2 * j + 1];
@@ -240,15 +241,16 @@ __global__ void __launch_bounds__(APPEND_THREADS, blocks_an_sm(sizeof(TI) == 2 &
     for (uint32_t r = row_off; r < rows; r += rows_at_once, src += rows_at_once * si0) {
         place_t const at = places[r];
         if (at.to < 0) continue;
-        float c[8];
+        float     c[8];
+        int const pairs = VEC ? 4 : HALVES ? t.n0 : min(4, (int)(p.rot - t.e0) / 2); // of the unit that are rotated (turn)
         if (turn) {
             float const* f = angles + at.angle;
             if (VEC) {
                 load_n<8, true>(f, c, 8);
             } else {
-                int const n = HALVES ? 2 * t.n0 : min(8, (int)(p.rot - t.e0));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) c[j] = j < n ? f[j] : (j & 1 ? 0.f : 1.f); // pairs that are not rotated stay what they are
+                for (int j = 0; j < 4; ++j)
+                    if (j < pairs) c[2 * j] = f[2 * j], c[2 * j + 1] = f[2 * j + 1];
             }
         }
         TI const* s = src;
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, blocks_an_sm(sizeof(TI) == 2 &
                 float     y[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[j] = to_f32(in[x].v[j]);
-                if (turn) rotate<HALVES>(y, c);
+                if (turn) rotate<HALVES>(y, c, pairs);
                 store_unit<HALVES, VEC>(to, t, y);
             }
             s += 2 * at_once * si1;

@@ -180,3 +180,31 @@ def test_null_tensors_are_refused(km):  # noqa: F811
         with pytest.raises(es.es_error) as e:
             km.cache_append(d, None, *[None if j == i else a for j, a in enumerate(args)])
         assert e.value.status == 6
+
+
+@pytest.mark.parametrize("rotary", [4, 12, 30])
+@pytest.mark.parametrize("pairing", ["adjacent", "halves"])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_elements_behind_the_rotated_part_are_copied(km, rotary, pairing, dtype):  # noqa: F811
+    """Bit for bit, whatever their neighbours are: infinities, NaN and zeros of either sign among them."""
+    b = batch_t([3], [9], 4, 2, 64, 16, dtype=dtype, seed=2, filler=0.25)
+    q, k, v, freqs = append_inputs(b, dtype, rotary, seed=1, packed=False)
+    for x in (q, k):
+        x[..., rotary + 1] = float("inf")
+        x[..., rotary + 2] = -0.0
+        x[..., rotary + 3] = -1.0
+        x[0, :, rotary + 5] = float("-inf")
+    want_q, want_k = q.clone(), k.clone()
+    b.to(DEV)
+    q, k, v, freqs = (t.to(DEV) for t in (q, k, v, freqs))
+    q_out = torch.zeros_like(q)
+    d = es.cache_append_t(cache_of(b), dtype, 4, q.stride()[:2], k.stride()[:2], v.stride()[:2], q_out.stride()[:2],
+                          freqs.shape[0], rotary, pairing)
+    km.cache_append(d, None, b.k_cache, b.v_cache, k, v, b.lengths, b.tables, b.row_offsets, freqs, q, q_out)
+    torch.cuda.synchronize()
+    assert km.device_status() == 0
+    bits = torch.int16 if dtype == "f16" else torch.int32
+    pages = b.tables[0].cpu().long()
+    got_k = torch.stack([b.k_cache.cpu()[pages[p // 16], p % 16] for p in range(9, 12)])
+    for got, want in ((q_out.cpu(), want_q), (got_k, want_k)):
+        assert torch.equal(got[..., rotary:].contiguous().view(bits), want[..., rotary:].contiguous().view(bits))
