@@ -51,26 +51,18 @@ template <> struct alignas(16) vec_t<__half, 8> { __half v[8]; };
 template <> struct alignas(8) vec_t<__half, 4> { __half v[4]; };
 template <> struct alignas(16) vec_t<float, 4> { float v[4]; };
 
-// N consecutive elements as f32; N = 8 or 4 with VEC (16-byte aligned rows), else one by one up to `n`
-template <int N, bool VEC, typename T> __device__ __forceinline__ void load_n(T const* p, float (&x)[N], int n)
+// 8 consecutive floats, 16-byte aligned
+__device__ __forceinline__ void load_8(float const* p, float (&x)[8])
 {
-    if constexpr (VEC && sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            vec_t<float, 4> t = *reinterpret_cast<vec_t<float, 4> const*>(p + i);
+    for (int i = 0; i < 8; i += 4) {
+        vec_t<float, 4> const t = *reinterpret_cast<vec_t<float, 4> const*>(p + i);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[i + j] = t.v[j];
-        }
-    } else if constexpr (VEC) {
-        vec_t<__half, N> t = *reinterpret_cast<vec_t<__half, N> const*>(p);
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = __half2float(t.v[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = j < n ? to_f32(p[j]) : 0.f;
+        for (int j = 0; j < 4; ++j) x[i + j] = t.v[j];
     }
 }
 
+// N consecutive elements from f32; N = 8 or 4 with VEC (aligned to their size, at most 16 bytes), else one by one up to `n`
 template <int N, bool VEC, typename T> __device__ __forceinline__ void store_n(T* p, float const (&x)[N], int n)
 {
     if constexpr (VEC && sizeof(T) == 4) {
@@ -246,7 +238,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, blocks_an_sm(sizeof(TI) == 2 &
         if (turn) {
             float const* f = angles + at.angle;
             if (VEC) {
-                load_n<8, true>(f, c, 8);
+                load_8(f, c);
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)

@@ -425,7 +425,7 @@ __device__ __forceinline__ finish_t finish(float m, float l, bool has_base, floa
     return f;
 }
 
-// W consecutive elements (4 or 2 or 1) of a finished row
+// W consecutive elements (4; of f16 also 2) of a finished row
 template <typename T, int W>
 __device__ __forceinline__ void write_out(paged_params_t const& p, int row, uint32_t head, uint32_t e, float const (&o)[W],
                                           finish_t const& f, bool aligned)
@@ -449,17 +449,13 @@ __device__ __forceinline__ void write_out(paged_params_t const& p, int row, uint
     T* d = static_cast<T*>(p.out) + (int64_t)row * p.out_stride[0] + (int64_t)head * p.out_stride[1] + e;
     if (aligned && e + W <= p.d) {
         if constexpr (sizeof(T) == 4) {
-            if constexpr (W == 4) *reinterpret_cast<float4*>(d) = make_float4(r[0], r[1], r[2], r[3]);
-            else if constexpr (W == 2) *reinterpret_cast<float2*>(d) = make_float2(r[0], r[1]);
-            else d[0] = r[0];
+            *reinterpret_cast<float4*>(d) = make_float4(r[0], r[1], r[2], r[3]);
         } else {
             if constexpr (W == 4) {
                 __half2 const a = __floats2half2_rn(r[0], r[1]), b = __floats2half2_rn(r[2], r[3]);
                 *reinterpret_cast<uint2*>(d) = make_uint2(*reinterpret_cast<uint32_t const*>(&a), *reinterpret_cast<uint32_t const*>(&b));
-            } else if constexpr (W == 2) {
-                *reinterpret_cast<__half2*>(d) = __floats2half2_rn(r[0], r[1]);
             } else {
-                from_f32(d[0], r[0]);
+                *reinterpret_cast<__half2*>(d) = __floats2half2_rn(r[0], r[1]);
             }
         }
         return;
