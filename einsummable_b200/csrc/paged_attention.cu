@@ -3,7 +3,8 @@
 //   s_j = scale q . k_j,   out = sum_j exp(s_j - lse) v_j,   lse = log sum_j exp(s_j)
 //
 // in one pass over the keys with the running maximum and sum of a softmax.  A shared prefix is attended first,
-// as one sequence whose rows are the rows of the whole batch -- its keys are read once for all of them --
+// as one sequence whose rows are the rows of the whole batch -- its keys are read once for a tile of them, which is
+// 8, 16 or 256 rows a key head on the tensor cores and 1 to 8 without --
 // into an f32 result and its lse; the sequences' own keys follow, and the two are weighed by exp(lse) where a
 // row is finished.
 #include <algorithm>
@@ -259,7 +260,7 @@ int choose(paged_params_t const& q, int dtype, bool vec, part_t (&c)[2])
     if (fewest <= MMA_MAX_TR) {
         p.packed_max = MMA_MAX_TR;
         uint32_t const rows = p.prefix_len >= 0 ? most : p.group; // of an item, where tokens come singly
-        // (tiles of 32 rows spill: 8 sequences of 4 query heads a key head behind 8000 tokens took 76 us, 41 with tcgen05)
+        // (tiles of 32 rows spill: 8 sequences of 4 query heads a key head behind 8000 tokens took 76 us, 45 with tcgen05)
         c[n++] = rows <= 8 ? mma_part<1>(p) : mma_part<2>(p);
     }
     if (most > MMA_MAX_TR) {
@@ -349,9 +350,12 @@ int launch_paged_attention(es_paged_attention_t const& a, es_paged_attention_arg
     bool const vec = aligned16(a, x);
     // A short prefix is read by every sequence for itself, in front of its own keys and out of the L2 cache: one
     // kernel and a join.  Reading it once adds two kernels -- few rows: the same kind again (8 sequences of 32 key
-    // heads behind 1000 tokens, 131 MB read in all: 25 us shared, 29 in front; 65 MB: equal), more: tcgen05's, whose
-    // start alone is worth some 20 us (16 sequences of 8 key heads behind 1000 / 2000 / 4000 tokens, 65 / 131 / 262
-    // MB: 37 / 37 / 37 us shared, 22 / 29 / 39 in front).  Single tokens only: parts of prompts have rows enough to
+    // heads behind 500 / 1000 / 2000 tokens, 62 / 125 / 250 MB read in all: 24 / 26 / 36 us shared, 18 / 32 / 42 in
+    // front; 3 sequences of 8 behind 4000, 47 MB: 36 and 26), more: tcgen05's, whose start alone is worth some 20 us
+    // (16 sequences of 8 key heads behind 1000 / 2000 / 4000 tokens, 62 / 125 / 250 MB: 38 / 38 / 40 us shared,
+    // 26 / 30 / 40 in front; 64 sequences behind 500 / 1000 / 2000, 125 / 250 / 500 MB: 46 / 46 / 46 and 34 / 44 /
+    // 63; 16 of 4 key heads of 64 behind 8000, 125 MB: 36 and 36).  f32, 4 key heads of 64: 8 sequences behind 4000,
+    // 62 MB, 42 and 38; 64 behind 2000, 250 MB, 99 and 95.  Single tokens only: parts of prompts have rows enough to
     // share.
     bool const     tc = c.dtype == ES_F16 && vec && c.head_dim <= 128;
     uint64_t const all = (uint64_t)c.batch * a.prefix_len * c.kv_heads * c.head_dim * 2 * dtype_size(c.dtype);

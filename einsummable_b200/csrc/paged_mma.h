@@ -13,7 +13,7 @@
 // accumulators rescaled, only when a score passes it by more than 2^4: one vote a tile, no reduction.
 // (With 16-row tiles, per-tile maxima and copy addresses formed anew for every copy a tile took 570
 // instructions and 1.6 us a warp, and 64 ragged sequences 117 us.)
-// Measured, 32 query heads on 8 key heads of 128: 2 x 131070 keys (1.07 GB) 171-176 us = 6.1-6.3 TB/s, 64 sequences of
+// Measured, 32 query heads on 8 key heads of 128: 2 x 131070 keys (1.07 GB) 175 us = 6.1 TB/s, 64 sequences of
 // 1 to 8192 tokens (252 MB) 51 us = 4.9 TB/s; 8 warps of 3 stages an SM (2 stages: 66 us for the ragged batch where
 // 3 took 62).
 #pragma once

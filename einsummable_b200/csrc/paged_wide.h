@@ -1,12 +1,14 @@
 // Paged attention for many packed rows a key head (a batch behind a shared prefix, parts of prompts), f16, on
 // the fifth-generation tensor cores.
 //
-// Bound: the tensor cores, and as much the exponentials: a tile of 128 rows x 128 keys of 128 elements is 2 * 512
-// cycles of products and, at 16 exponentials a cycle, 1024 of softmax.  (Measured: 1330 and 1940 with what lies between
-// them, 3500 for the pair of tiles; 256 rows a key head behind 16000 shared tokens 16.9 GF in 31 us, a prompt of 4096
-// tokens with 32 heads 137 GF in 172 us = 0.80 PFLOP/s, where the first tile of a block alone takes 5 us.)  So an item is two tiles of 128 packed rows
-// that share the keys in shared memory and take turns: while one tile's scores are on the tensor cores, the
-// other's are exponentials.  One persistent block an SM, 20 warps:
+// Bound: the tensor cores, and nearly as much the exponentials: a tile of 128 rows x 128 keys of 128 elements is 512
+// cycles of scores and 2 * 512 of values (P has two parts) and, at 16 exponentials a cycle, 1024 of softmax.  (Measured:
+// 2240 from the scores to P and 1990 from P to the next scores, a chain of 4230 in which the other tile of the pair has
+// its turn, 3072 of them products; 256 rows a key head behind 16000 shared tokens 38 us, a prompt of 4096 tokens with 32
+// heads 137 GF in 208 us = 0.66 PFLOP/s.  A block's start -- counting the work, its first tile -- is 23000 cycles behind
+// a prefix and 41000 with row offsets, much of it waiting for instructions; an item's result 4000.)  So an item is two
+// tiles of 128 packed rows that share the keys in shared memory and take turns: while one tile's scores are on the tensor
+// cores, the other's are exponentials.  One persistent block an SM, 20 warps:
 //   warps 0-7, 8-15  softmax of tile 0 / 1, two threads a row (= TMEM lane), 64 keys each -- half the
 //                    chain of one thread a row, and half the time results take to leave: the maximum of the scores, the
 //                    accumulator rescaled when it has moved by more than 2^4, then the exponentials (f32) against it,
@@ -20,9 +22,10 @@
 //                    values.  (With every row's address sent through a shuffle a tile's 64 KB took 8700 cycles.)
 // TMEM: scores 2 x 128 columns, accumulators 2 x 128.  Products of one thread are done in order, so S_t of the
 // next tile may be issued over P_t as soon as P_t V is, and whoever sees S_t complete knows P_t V to be.
-// Tried and dropped: a third of the exponentials as polynomials on the fused multiply-add units (a 4096-token prompt
-// 171 -> 186 us), P handed over in halves (the same), a first pass over an empty tile to warm the instruction cache
-// (64 sequences behind 16000 tokens 60 -> 66 us).
+// Tried and dropped, with P in one part: a third of the exponentials as polynomials on the fused multiply-add units (a
+// 4096-token prompt 171 -> 186 us), P handed over in halves (the same), a first pass over an empty tile to warm the
+// instruction cache (64 sequences behind 16000 tokens 60 -> 66 us).  With two: half of the scores kept in registers
+// between the two passes (the prompt 210 -> 222), all 64 loaded at once for the maximum (208 -> 215).
 // Every wait is bounded; on expiry the kernel records 0x31-0x39, lets its copies land, frees TMEM and returns.
 #pragma once
 #include "paged_mma.h"

@@ -237,7 +237,7 @@ class kernel_manager_t:
     def prefix_attention(self, desc, stream, out, q, k_cache, v_cache, prefix_pages, lengths, tables, row_offsets=None,
                          lse=None, workspace=None):
         """The same behind a prefix that all sequences share: its desc.prefix_len tokens lie in the pages
-        prefix_pages (int32 on the device) and are read once for the whole batch."""
+        prefix_pages (int32 on the device) and are read for many rows at once."""
         x = _pack9(_adr(q), _adr(k_cache), _adr(v_cache), _adr(out), _adr(lse), _adr(row_offsets), _adr(lengths), _adr(tables),
                    _adr(prefix_pages))
         ws, n = (None, 0) if workspace is None else (_ptr(workspace[0]), int(workspace[1]))

@@ -334,8 +334,9 @@ int es_b200_launch_cache_append(es_b200_t* h, const es_cache_append_t* a, const 
  * without a key to see, NaN and infinities concern the rows that see them only -- and, on the tensor cores, the
  * earlier rows of the same call in the same sequence, for which they are 0 times the value.
  * prefix_len tokens, the same for all sequences and listed by prefix_pages, can lie in front of every
- * sequence's own (es_b200_launch_prefix_attention): every row sees all of them, and they are read once
- * for the whole batch.  lengths and tables then count a sequence's own tokens only.
+ * sequence's own (es_b200_launch_prefix_attention): every row sees all of them, and they are read once for
+ * up to 256 rows of a key head together (on the tensor cores; without them for up to 8) -- or, where that is
+ * little, by each sequence.  lengths and tables then count a sequence's own tokens only.
  * The workspace (es_b200_paged_attention_workspace; 16-byte aligned, contents irrelevant before and
  * after) may be shared by calls that do not overlap in time.  out may not overlap q or the cache.  The same
  * call gives the same bits.  Make one call on a device before capturing one. */
