@@ -160,19 +160,22 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) paged_wide_kernel(const __gri
         ctrl->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (p.d != DPAD) // columns that no copy fills: zeros
+        for (uint32_t i = threadIdx.x * 16; i < 6 * TILE; i += WIDE_THREADS * 16)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sQ + i), "r"(0) : "memory");
+    // TMEM is taken when the kernel before is done (ORDER_LATE: that one belongs to this call, and holds what it needs), and
+    // the next one may start when it is taken: a kernel that waits for another never holds what that one still has to take.
+    if (p.order != ORDER_LATE) ES_PDL_WAIT();
     if (warp == WIDE_SOFTMAX_WARPS) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctrl->tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (p.d != DPAD) // columns that no copy fills: zeros
-        for (uint32_t i = threadIdx.x * 16; i < 6 * TILE; i += WIDE_THREADS * 16)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sQ + i), "r"(0) : "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     uint32_t const tmem = ctrl->tmem_base; // scores: + 128 t; accumulators: + 256 + 128 t
-    begin_order(p);
+    asm volatile("griddepcontrol.launch_dependents;");
     work_t w;
     find_work<TR, BK, OVH, WIDE_THREADS, 1>(p, w, sched);
 
