@@ -176,9 +176,20 @@ __device__ __forceinline__ place_t find_place(append_params_t const& p, uint32_t
         for (uint32_t i0 = 0; i0 < p.batch; i0 += 32)
             seq += __popc(__ballot_sync(0xffffffffu, i0 + lane < p.batch && p.row_offsets[i0 + lane + 1] <= (int)row));
         if (seq >= (int)p.batch) return t; // padding
-        int const a = p.row_offsets[seq], b = p.row_offsets[seq + 1];
+        int  a = p.row_offsets[seq], b = p.row_offsets[seq + 1];
+        auto holds = [&] { return a >= 0 && a <= (int)row && b > (int)row && b <= (int)p.rows; };
+        if (!holds()) { // offsets that fall, or pass the rows: the first sequence that holds the row nonetheless
+            report(PAGED_BAD_ROWS);
+            seq = -1;
+            for (uint32_t i0 = 0; i0 < p.batch && seq < 0; i0 += 32) {
+                if (i0 + lane < p.batch) a = p.row_offsets[i0 + lane], b = p.row_offsets[i0 + lane + 1];
+                seq = __ffs(__ballot_sync(0xffffffffu, i0 + lane < p.batch && holds())) - 1;
+                if (seq >= 0) seq += (int)i0;
+            }
+            if (seq < 0) return t;
+            b = p.row_offsets[seq + 1];
+        }
         back = b - (int)row;
-        if (a < 0 || a > (int)row || back <= 0 || b > (int)p.rows) return report(PAGED_BAD_ROWS); // offsets that fall, or pass the rows
     }
     int const length = p.lengths[seq];
     if (length < 0 || (uint32_t)length > p.capacity) return report(PAGED_BAD_LENGTH);
@@ -214,6 +225,11 @@ __global__ void __launch_bounds__(APPEND_THREADS, blocks_an_sm(sizeof(TI) == 2 &
         place_t const w = find_place(p, row0 + r, what);
         if ((threadIdx.x & 31) == 0) places[r] = w;
     }
+    if (blockIdx.x == 0 && p.row_offsets) // wrong offsets that no row meets are reported too
+        for (uint32_t i = threadIdx.x; i < p.batch; i += APPEND_THREADS) {
+            int const a = p.row_offsets[i], b = p.row_offsets[i + 1];
+            if (a < 0 || b < a || b > (int)p.rows) atomicCAS(&g_append_error, 0u, (unsigned)PAGED_BAD_ROWS);
+        }
     uint32_t const heads = what ? p.kv_heads : p.heads;
     uint32_t const at_once = APPEND_THREADS / p.upd.d; // heads that the block moves at once: of one row, or of several rows
     uint32_t const mine = fdivide(threadIdx.x, p.upd), u = threadIdx.x - mine * p.upd.d;

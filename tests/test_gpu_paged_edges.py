@@ -208,3 +208,27 @@ def test_elements_behind_the_rotated_part_are_copied(km, rotary, pairing, dtype)
     got_k = torch.stack([b.k_cache.cpu()[pages[p // 16], p % 16] for p in range(9, 12)])
     for got, want in ((q_out.cpu(), want_q), (got_k, want_k)):
         assert torch.equal(got[..., rotary:].contiguous().view(bits), want[..., rotary:].contiguous().view(bits))
+
+
+@pytest.mark.parametrize("many", [1, 30])
+def test_append_with_bad_row_offsets_serves_the_other_sequences(km, many):  # noqa: F811
+    """Sequences whose rows the offsets name are appended, wherever the wrong entries stand; nothing else is written."""
+    for off, valid in [([0, 2, 5, 99], [0, 1]), ([0, 2, 5, 3], [0, 1]), ([-1, 2, 3, 5], [1, 2]), ([0, 2, 2 ** 20, 5], [0]),
+                       ([0, 2, 5, -7], [0, 1]), ([0, 3, 1, 0], [0]), ([2, 5, 0, 0], [0])]:
+        off = [x * many for x in off]
+        b = batch_t([2 * many, many, 2 * many], [40, 200, 90], 4, 2, 64, 16, seed=9, filler=0.25)
+        q, k, v, _ = append_inputs(b, "f16", 64, seed=8, packed=False)
+        want = b.v_cache.clone()
+        for i in valid:
+            n = off[i + 1] - off[i]
+            for r in range(n):
+                p = b.total[i] - n + r
+                want[b.tables[i, p // 16].long(), p % 16] = v[off[i] + r]
+        b.to(DEV)
+        k, v = k.to(DEV), v.to(DEV)
+        b.row_offsets = torch.tensor(off, dtype=torch.int32, device=DEV)
+        d = es.cache_append_t(cache_of(b), "f16", 0, k_stride=k.stride()[:2], v_stride=v.stride()[:2])
+        km.cache_append(d, None, b.k_cache, b.v_cache, k, v, b.lengths, b.tables, b.row_offsets)
+        torch.cuda.synchronize()
+        assert km.device_status() == 0x23
+        assert torch.equal(b.v_cache.cpu(), want)
