@@ -4,7 +4,7 @@
 // Bound: the tensor cores, and nearly as much the exponentials: a tile of 128 rows x 128 keys of 128 elements is 512
 // cycles of scores and 2 * 512 of values (P has two parts) and, at 16 exponentials a cycle, 1024 of softmax.  (Measured:
 // 2240 from the scores to P and 1990 from P to the next scores, a chain of 4230 in which the other tile of the pair has
-// its turn, 3072 of them products; 256 rows a key head behind 16000 shared tokens 38 us, a prompt of 4096 tokens with 32
+// its turn, 2 x 1536 of them products; 256 rows a key head behind 16000 shared tokens 38 us, a prompt of 4096 tokens with 32
 // heads 137 GF in 208 us = 0.66 PFLOP/s.  A block's start -- counting the work, its first tile -- is 23000 cycles behind
 // a prefix and 41000 with row offsets, much of it waiting for instructions; an item's result 4000.)  So an item is two
 // tiles of 128 packed rows that share the keys in shared memory and take turns: while one tile's scores are on the tensor
